@@ -8,7 +8,10 @@ CSRC = os.path.join(HERE, 'csrc')
 SO = os.path.join(HERE, 'libadvmix_hip.so')
 SOURCES = ['conv_mfma.hip', 'conv_direct.hip', 'conv_wino.hip', 'conv_wino4.hip', 'conv_smap.hip', 'conv_pw.hip', 'wgrad_direct.hip', 'wgrad_lds.hip', 'wgrad_wino.hip', 'norm.hip', 'pointwise.hip', 'advmix_ops.hip', 'postproc.hip', 'inputpipe.hip', 'nms.hip']
 FLAGS = ['-O3', '--offload-arch=gfx950', '-fPIC', '-munsafe-fp-atomics', '-std=c++17',
-         '-Wno-unused-result', '-Wno-pass-failed']     # (pass-failed: 'occupancy target not met' where LDS, not registers, is the limit)
+         '-Wno-unused-result', '-Wno-pass-failed',     # (pass-failed: 'occupancy target not met' where LDS, not registers, is the limit)
+         # No packed fp32 instructions (v_pk_fma_f32 and its like): the compiler makes them of ordinary float code, and some
+         # of their forms have given wrong results now and then.  (hipcc's host pass says that it does not know the feature.)
+         '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # Every kernel must fit its registers: a kernel with scratch (spilled VGPRs) is refused - none of the library's kernels needs
 # any, a spill is always an accident of a register cap, and spilling builds were among the suspects of round 3's
 # two-process NaN hunt (conv_direct.hip, at its launch bounds).  The compiler reports each kernel's scratch; the build reads it.
@@ -85,7 +88,7 @@ def build(force=False, verbose=True):
         _, err = p.communicate()
         other = [ln for ln in err.splitlines() if 'kernel-resource-usage' not in ln]
         # (the remark lines carry a source excerpt each: print only what is not part of the resource report)
-        msgs = [ln for ln in other if 'warning' in ln or 'error' in ln]
+        msgs = [ln for ln in other if ('warning' in ln or 'error' in ln) and 'packed-fp32-ops' not in ln]
         if msgs and verbose:
             print('\n'.join(msgs), flush=True)
         if p.returncode != 0:
