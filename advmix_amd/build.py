@@ -6,7 +6,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 SO = os.path.join(HERE, 'libadvmix_hip.so')
-SOURCES = ['conv_mfma.hip', 'conv_direct.hip', 'conv_wino.hip', 'conv_wino4.hip', 'conv_smap.hip', 'conv_pw.hip', 'wgrad_direct.hip', 'wgrad_lds.hip', 'wgrad_wino.hip', 'norm.hip', 'pointwise.hip', 'advmix_ops.hip', 'postproc.hip', 'inputpipe.hip', 'nms.hip']
+SOURCES = ['conv_mfma.hip', 'conv_direct.hip', 'conv_wino.hip', 'conv_wino4.hip', 'conv_smap.hip', 'conv_pw.hip', 'wgrad_direct.hip', 'wgrad_lds.hip', 'wgrad_wino.hip', 'norm.hip', 'layer_norm.hip', 'pointwise.hip', 'advmix_ops.hip', 'adamw.hip', 'postproc.hip', 'inputpipe.hip', 'nms.hip']
 FLAGS = ['-O3', '--offload-arch=gfx950', '-fPIC', '-munsafe-fp-atomics', '-std=c++17',
          '-Wno-unused-result', '-Wno-pass-failed',     # (pass-failed: 'occupancy target not met' where LDS, not registers, is the limit)
          # No packed fp32 instructions (v_pk_fma_f32 and its like): the compiler makes them of ordinary float code, and some

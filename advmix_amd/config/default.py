@@ -105,7 +105,8 @@ _DEFAULTS = {
                 'VAL_PARSING': False},
     'TRAIN': {'LR_FACTOR': 0.1, 'LR_STEP': [90, 110], 'LR': 0.001, 'OPTIMIZER': 'adam', 'MOMENTUM': 0.9,
               'WD': 0.0001, 'NESTEROV': False, 'GAMMA1': 0.99, 'GAMMA2': 0.0, 'BEGIN_EPOCH': 0,
-              'END_EPOCH': 140, 'RESUME': False, 'CHECKPOINT': '', 'BATCH_SIZE_PER_GPU': 32, 'SHUFFLE': True},
+              'END_EPOCH': 140, 'RESUME': False, 'CHECKPOINT': '', 'BATCH_SIZE_PER_GPU': 32, 'SHUFFLE': True,
+              'STATE_BITS': 32, 'CLIP_NORM': 0.0},              # (OPTIMIZER 'adamw' only: utils.get_optimizer)
     'TEST': {'BATCH_SIZE_PER_GPU': 32, 'FLIP_TEST': False, 'POST_PROCESS': False, 'SHIFT_HEATMAP': False,
              'USE_GT_BBOX': False, 'TEST_ROBUST': False, 'CORRUPTION_TYPE': '', 'IMAGE_THRE': 0.1,
              'NMS_THRE': 0.6, 'SOFT_NMS': False, 'OKS_THRE': 0.5, 'IN_VIS_THRE': 0.0, 'COCO_BBOX_FILE': '',

@@ -1159,6 +1159,130 @@ class InstanceNorm:
         return (dx,)
 
 
+_LN_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # ADVMIX_F32 / BF16 / F16
+
+
+def _row_stride(t):
+    """Elements between the rows of ``t`` (logical NCHW for 4-D, channels last otherwise) if its channels are neighbours and
+    all its rows lie at one distance, else None."""
+    if t.dim() == 4:
+        t = t.permute(0, 2, 3, 1)
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        return None
+    step = None                                            # walk outwards: every dimension must continue the one inside it
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n == 1:
+            continue
+        if step is None:
+            step, span = s, s * n
+        elif s != span:
+            return None
+        else:
+            span *= n
+    return t.shape[-1] if step is None else step
+
+
+class LayerNorm:
+    """y = (x - mean) / sqrt(var + eps) * gamma + beta over the channels: dim 1 of a 4-D NCHW map, the last dimension of
+    tokens [..., C].  tensors = (x, gamma | None, beta | None); meta = eps.  x in fp32, bf16 or fp16 (y and its gradient have
+    x's type), gamma and beta fp32.  Rows may lie apart (a slice of wider tokens); other layouts are copied first."""
+    NHWC = (0,)
+
+    @staticmethod
+    def accept(t):
+        if t.dtype not in _LN_TYPES or not t.is_cuda:
+            raise TypeError('layer_norm needs fp32, bf16 or fp16 CUDA tensors (no CPU fallback), got %s on %s' % (t.dtype, t.device))
+        if not 1 <= t.dim() <= 4:
+            raise ValueError('layer_norm: expected tokens [..., C] with up to 3 dimensions or a 4-D NCHW map, got %d-D' % t.dim())
+
+    @staticmethod
+    def LAYOUT(t):
+        """What GroupFn does to x and to dy BEFORE the lanes fork: checks, and a dense copy if the rows do not line up."""
+        LayerNorm.accept(t)
+        if _row_stride(t) is None:
+            t = keep(t.contiguous(memory_format=_CL if t.dim() == 4 else torch.contiguous_format))
+        return t
+
+    @staticmethod
+    def _sizes(x):
+        C = x.shape[1] if x.dim() == 4 else x.shape[-1]
+        return (x.numel() // C if C else 0), C
+
+    @staticmethod
+    def _like(x):
+        if x.dim() == 4:
+            B, C, H, W = x.shape
+            return torch.empty((B, H, W, C), device=x.device, dtype=x.dtype).permute(0, 3, 1, 2)
+        return torch.empty(x.shape, device=x.device, dtype=x.dtype)
+
+    @staticmethod
+    def check(x, gamma, beta, eps):
+        rows, C = LayerNorm._sizes(x)
+        if C == 0:
+            raise ValueError('layer_norm: no channels to normalise over')
+        if not (eps >= 0 and eps < float('inf')):
+            raise ValueError('layer_norm: eps must be finite and not negative, got %r' % (eps,))
+        for name, p in (('gamma', gamma), ('beta', beta)):
+            if p is None:
+                continue
+            if p.dtype != torch.float32 or p.device != x.device:
+                raise TypeError('layer_norm: %s must be fp32 on %s, got %s on %s' % (name, x.device, p.dtype, p.device))
+            if p.shape != (C,) or not p.is_contiguous():
+                raise ValueError('layer_norm: %s must be a contiguous [%d], got %s' % (name, C, list(p.shape)))
+            if p.requires_grad and not p.is_leaf:          # its gradient is accumulated into .grad, which only a leaf has
+                raise ValueError('layer_norm: %s requires a gradient but is not a leaf (parameter)' % name)
+
+    @staticmethod
+    def fwd(st, lane, t, meta, needs):
+        x, gamma, beta = t
+        x = LayerNorm.LAYOUT(x)
+        LayerNorm.check(x, gamma, beta, meta)
+        rows, C = LayerNorm._sizes(x)
+        y = LayerNorm._like(x)
+        mean = rstd = None
+        if any(needs):
+            mean, rstd = torch.empty(2, rows, device=x.device, dtype=torch.float32).unbind(0)
+        if rows:
+            call('advmix_layer_norm_fwd', _p(x), _row_stride(x), _p(gamma), _p(beta), _p(y), _p(mean), _p(rstd), rows, C,
+                 _LN_TYPES[x.dtype], meta, st)
+        return (y,), (() if mean is None else (x, gamma, beta, mean, rstd)), None
+
+    @staticmethod
+    def bwd(st, lane, saved, extra, meta, grads, needs):
+        if torch.is_grad_enabled():
+            raise RuntimeError('advmix_amd: layer_norm has no second derivative (backward with create_graph=True)')
+        x, gamma, beta, mean, rstd = saved
+        dy = LayerNorm.LAYOUT(grads[0])
+        rows, C = LayerNorm._sizes(x)
+        dx = LayerNorm._like(x) if needs[0] else None
+        dg = LayerNorm._grad(gamma, st) if needs[1] else None
+        db = LayerNorm._grad(beta, st) if needs[2] else None
+        if rows:
+            kind = _LN_TYPES[x.dtype]
+            part = None
+            if dg is not None or db is not None:           # (this call's own: two captured graphs must not share it)
+                n = lib.advmix_layer_norm_parts(rows, C, kind)
+                part = keep(torch.empty(n * 2 * C, device=x.device, dtype=torch.float32))
+            call('advmix_layer_norm_bwd', _p(dy), _row_stride(dy), _p(x), _row_stride(x), _p(gamma), _p(mean), _p(rstd), _p(dx),
+                 _p(dg), _p(db), _p(part), rows, C, kind, st)
+        return dx, None, None
+
+    @staticmethod
+    def _grad(p, st):
+        g = _grad_buf(p, st)
+        if g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape or g.device != p.device:
+            raise RuntimeError('layer_norm: a parameter\'s .grad must be a contiguous fp32 tensor of its shape')
+        return g
+
+    @staticmethod
+    def before_bwd(saved, needs, st):
+        """Groups of several members: the gradient buffers exist before the lanes fork, so that members that share a
+        parameter add to ONE buffer (the additions themselves are atomic)."""
+        for p, need in zip(saved[1:3], needs[1:3]):
+            if need:
+                LayerNorm._grad(p, st)
+
+
 class Act:
     NHWC = (0,)      # inputs made dense NHWC BEFORE the lanes fork (None = all)
     @staticmethod
@@ -1709,7 +1833,7 @@ class GroupFn(torch.autograd.Function):
             idx = op.NHWC(meta) if callable(op.NHWC) else op.NHWC
             for k in (range(cnt) if idx is None else idx):
                 if flat[pos + k] is not None:
-                    flat[pos + k] = nhwc(flat[pos + k])
+                    flat[pos + k] = getattr(op, 'LAYOUT', nhwc)(flat[pos + k])
             pos += cnt
         _ensure_workspaces(dev, nl)
         needs_all = ctx.needs_input_grad[1:]
@@ -1751,11 +1875,18 @@ class GroupFn(torch.autograd.Function):
         members = ctx.members
         nl = min(len(members), MAX_LANES)
         cur = torch.cuda.current_stream(dev)
-        gouts = [nhwc(g) if (g is not None and g.dim() == 4) else g for g in gouts]   # before the fork
-        _ensure_workspaces(dev, nl)
         grads = [None] * ctx.n_in
         needs_all = ctx.needs_input_grad[1:]
         spans, extras = ctx.spans, ctx.extras
+        gouts = list(gouts)
+        for (op, _, _), (ipos, icnt, opos, ocnt, spos, scnt) in zip(members, spans):   # before the fork
+            own = getattr(op, 'LAYOUT', None)
+            for k in range(opos, opos + ocnt):
+                if gouts[k] is not None and (own is not None or gouts[k].dim() == 4):
+                    gouts[k] = (own or nhwc)(gouts[k])
+            if nl > 1 and hasattr(op, 'before_bwd') and any(g is not None for g in gouts[opos:opos + ocnt]):
+                op.before_bwd(saved[spos:spos + scnt], needs_all[ipos:ipos + icnt], ctypes.c_void_p(cur.cuda_stream))
+        _ensure_workspaces(dev, nl)
 
         def run_member(i, handle, lane):
             op, cnt, meta = members[i]
@@ -1825,6 +1956,17 @@ def conv_bn(x, w, gamma, beta, rmean, rvar, nbt, residual=None, stride=1, pad=0,
 
 def instance_norm(x, act=ACT_NONE, eps=1e-5):
     return _one(InstanceNorm, (x,), (act, eps))
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-5):
+    """Layer norm over dim 1 of a 4-D NCHW map (channels_last memory: every pixel by itself) or over the last dimension of
+    tokens [..., C] (1-D to 3-D).  x: fp32, bf16 or fp16; gamma, beta: fp32 [C] parameters or None.  The statistics and the
+    parameters' gradients are summed in fp32 in a fixed order; those gradients are accumulated into ``.grad`` as everywhere
+    here.  No second derivative.  As with any op here, capture a backward pass into a HIP graph only when no eager autograd
+    graph of the same leaves is alive."""
+    LayerNorm.accept(x)                                    # (refuses a CPU tensor before its device is made current)
+    with torch.cuda.device(x.device):
+        return _one(LayerNorm, (x, gamma, beta), eps)
 
 
 def activation(x, act):

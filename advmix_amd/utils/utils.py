@@ -238,14 +238,242 @@ class FlatSGD(FlatAdam):
         self.sync_hyper()
 
 
+class FlatAdamW(FlatAdam):
+    """torch.optim.AdamW(params, lr, betas, eps, weight_decay) semantics on FlatAdam's flat buffers, with parameter groups,
+    a step that clips the gradient by its global norm, and moments in 32 or in 8 bits.
+
+    ``params``: parameters, or groups (dicts with their own lr / betas / eps / weight_decay).  Every parameter takes the step,
+    one whose gradient is zero too: it decays.
+    ``max_norm``: the gradients count as g * min(1, max_norm / (|g| + 1e-6)), |g| the 2-norm over all of them; ``p.grad`` keeps
+    what the backward pass left, the norm before clipping is in ``grad_norm`` (device) after a step.
+    ``state_bits`` 8: 2 bytes of state per parameter instead of 8 - m and sqrt(v) as e4m3 numbers, blocks of 256 elements of a
+    tensor (in memory order) with a power of two as their scale, rounded up or down by a hash of place, step and ``seed`` so that
+    small steps count on average.  The same seed gives the same bits in every replica and after a resume.
+    ``state_dict`` holds exp_avg / exp_avg_sq as torch.optim does, or with 8 bits exp_avg_codes / exp_avg_scale and
+    exp_avg_root_codes / exp_avg_root_scale as they are; either kind of optimizer loads either kind of state."""
+
+    CHUNK, BLOCK, HYPER, PARTS = 1024, 256, 8, 1024
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError('FlatAdamW: state_bits must be 8 or 32, got %r' % (state_bits,))
+        if not 0 <= int(seed) < 2 ** 31:
+            raise ValueError('FlatAdamW: seed must be in [0, 2^31), got %r' % (seed,))
+        self.state_bits, self.seed = state_bits, int(seed)
+        self._clips = max_norm is not None
+        self.max_norm = max_norm
+        self._flat = None
+        torch.optim.Optimizer.__init__(self, params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False))
+        self._check()
+        if all(p.is_cuda for p in self._params()):
+            self._ensure_flat()
+
+    def add_param_group(self, group):
+        if self._flat is not None:
+            raise RuntimeError('FlatAdamW: the flat buffers are laid out; give every group to the constructor')
+        super().add_param_group(group)
+
+    def _check(self):
+        ps = self._params()
+        if len(set(map(id, ps))) != len(ps):
+            raise ValueError('FlatAdamW: a parameter was given twice')
+        if len({p.device for p in ps}) > 1:
+            raise ValueError('FlatAdamW: the parameters are on different devices')
+        for p in ps:
+            if p.dtype != torch.float32:
+                raise TypeError('FlatAdamW handles fp32 parameters only')
+            if not p.requires_grad:
+                raise ValueError('FlatAdamW: a parameter does not require a gradient (it would decay all the same): leave it out')
+        if not any(p.numel() for p in ps):
+            raise ValueError('FlatAdamW: no elements to train')
+        self._hyper_tuple()
+
+    def _hyper_tuple(self):
+        """One row of doubles per group behind one for the whole step, checked."""
+        if (self.max_norm is not None) != self._clips:
+            raise ValueError('FlatAdamW: whether the step clips is decided by the constructor')
+        if self._clips and not 0 < float(self.max_norm) < float('inf'):
+            raise ValueError('FlatAdamW: max_norm must be positive and finite, got %r' % (self.max_norm,))
+        rows = [float(self.max_norm) if self._clips else 0.0] + [0.0] * (self.HYPER - 1)
+        for g in self.param_groups:
+            lr, (b1, b2), eps, wd = float(g['lr']), g['betas'], float(g['eps']), float(g['weight_decay'])
+            if g.get('amsgrad') or g.get('maximize'):
+                raise ValueError('FlatAdamW: amsgrad and maximize are not supported')
+            if not (0 <= lr < float('inf') and 0 <= b1 < 1 and 0 <= b2 < 1 and 0 <= wd < float('inf')):
+                raise ValueError('FlatAdamW: lr and weight_decay must be finite and not negative, betas in [0, 1): got %r'
+                                 % ((lr, b1, b2, wd),))
+            if not 1e-38 < eps < float('inf'):               # (an element that never had a gradient is 0 / eps, not 0 / 0)
+                raise ValueError('FlatAdamW: eps must be positive in fp32, got %r' % (eps,))
+            rows += [lr, float(b1), float(b2), eps, wd] + [0.0] * (self.HYPER - 5)
+        return tuple(rows)
+
+    def _ensure_flat(self):
+        if self._flat is not None:
+            return
+        super()._ensure_flat()
+        fp, _, m, v = self._flat
+        dev = fp.device
+        group = {id(p): k for k, g in enumerate(self.param_groups) for p in g['params']}
+        rows, self._chunks, self._blocks, block = [], [], [], 0
+        for p, off in zip(self._params(), self._offsets):
+            n = _ceil4(p.numel())
+            first, first_block = len(rows), block
+            for k in range(0, n, self.CHUNK):
+                rows.append((off + k, min(self.CHUNK, n - k), group[id(p)], block + k // self.BLOCK))
+            block += -(-n // self.BLOCK)
+            self._chunks.append((first, len(rows)))
+            self._blocks.append((first_block, block))
+        self._table = torch.tensor(rows, dtype=torch.int64).to(dev)
+        self._hyper = torch.tensor(self._hyper_host, dtype=torch.float64).to(dev)
+        self._coef = torch.zeros(8 * len(self.param_groups) + 8, device=dev, dtype=torch.float32)
+        self._parts = torch.empty(self.PARTS, device=dev, dtype=torch.float64) if self._clips else None
+        self.grad_norm = torch.zeros((), device=dev, dtype=torch.float32) if self._clips else None
+        if self.state_bits == 8:
+            self._flat = self._flat[:2] + tuple(torch.zeros(fp.numel(), device=dev, dtype=torch.uint8) for _ in range(2))
+            self._scales = tuple(torch.zeros(block, device=dev, dtype=torch.uint8) for _ in range(2))
+
+    def flat_state(self):
+        """[parameters, m, v, step]; with 8 bits [parameters, m codes, r codes, step, m exponent bytes, r exponent bytes]."""
+        return super().flat_state() + (list(self._scales) if self.state_bits == 8 else [])
+
+    def sync_hyper(self):
+        self._ensure_flat()
+        cur = self._hyper_tuple()
+        if cur != self._hyper_host:
+            self._hyper.copy_(torch.tensor(cur, dtype=torch.float64))
+            self._hyper_host = cur
+
+    def zero_grad(self, set_to_none=False):
+        self._ensure_flat()
+        with torch.cuda.device(self._flat[0].device):
+            super().zero_grad(set_to_none)
+
+    @torch.no_grad()
+    def step(self, closure=None, sync_hyper=True):
+        if closure is not None:
+            raise ValueError('FlatAdamW: step() takes no closure')
+        self._ensure_flat()
+        if sync_hyper and not torch.cuda.is_current_stream_capturing():
+            self.sync_hyper()
+        self._attach_grads(strict=True)
+        fp, fg, m, v = self._flat
+        P = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())       # noqa: E731
+        with torch.cuda.device(fp.device):
+            st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+            if self._clips:
+                call('advmix_grad_sumsq', P(fg), fg.numel(), P(self._parts), self.PARTS, st)
+            rest = (P(self._table), len(self._table), P(self._hyper), len(self.param_groups), P(self._step), P(self._parts),
+                    self.PARTS if self._clips else 0, P(self.grad_norm))
+            if self.state_bits == 8:
+                call('advmix_adamw8', P(fp), P(fg), P(m), P(v), P(self._scales[0]), P(self._scales[1]), *rest, self.seed,
+                     P(self._coef), st)
+            else:
+                call('advmix_adamw', P(fp), P(fg), P(m), P(v), *rest, P(self._coef), st)
+
+    # ---- state ------------------------------------------------------------------------------
+    _KEYS = (('exp_avg', 'exp_avg_codes', 'exp_avg_scale'), ('exp_avg_sq', 'exp_avg_root_codes', 'exp_avg_root_scale'))
+
+    def state_dict(self):
+        self._ensure_flat()
+        step, state, at = float(self._step.item()), {}, 0
+        for i, (p, off) in enumerate(zip(self._params(), self._offsets)):
+            state[i] = {'step': torch.tensor(step)}
+            for k, (full, codes, scale) in enumerate(self._KEYS):
+                own = self._view(self._flat[2 + k], off, p).detach().clone()
+                if self.state_bits == 32:
+                    state[i][full] = own
+                else:
+                    lo, hi = self._blocks[i]
+                    state[i][codes] = own.view(torch.float8_e4m3fn)
+                    state[i][scale] = self._scales[k][lo:hi].clone().view(torch.float8_e8m0fnu)
+        groups = []
+        for g in self.param_groups:
+            groups.append(dict({k: v for k, v in g.items() if k != 'params'}, params=list(range(at, at + len(g['params'])))))
+            at += len(g['params'])
+        return {'state': state, 'param_groups': groups}
+
+    def load_state_dict(self, sd):
+        self._ensure_flat()
+        ps, fp = self._params(), self._flat[0]
+        sizes = [len(g['params']) for g in sd['param_groups']]
+        if sizes != [len(g['params']) for g in self.param_groups]:
+            raise ValueError('FlatAdamW: the state has other parameter groups (%r parameters)' % (sizes,))
+        todo = []
+        for i, p in enumerate(ps):                            # check everything before anything is overwritten
+            st = sd['state'].get(i) or sd['state'].get(str(i))
+            if st is None:
+                continue
+            lo, hi = self._blocks[i]
+            for full, codes, scale in self._KEYS:
+                if full in st:
+                    if st[full].shape != p.shape:
+                        raise ValueError('FlatAdamW: %s of parameter %d has another shape' % (full, i))
+                elif codes not in st or scale not in st or st[codes].shape != p.shape or st[scale].numel() != hi - lo:
+                    raise ValueError('FlatAdamW: the state of parameter %d lacks %s, or its codes have another shape' % (i, full))
+            todo.append((i, p, st))
+        before = [dict(g) for g in self.param_groups]
+        for g, new in zip(self.param_groups, sd['param_groups']):
+            g.update({k: v for k, v in new.items() if k != 'params'})
+        try:
+            self._hyper_tuple()
+        except ValueError:
+            for g, old in zip(self.param_groups, before):
+                g.update(old)
+            raise
+        step = 0
+        byte = lambda t: t.view(torch.uint8) if t.element_size() == 1 else t          # noqa: E731
+        P = lambda t, at=0: ctypes.c_void_p(t.data_ptr() + at)          # noqa: E731
+        with torch.no_grad(), torch.cuda.device(fp.device):
+            st_ = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+            other = [None, None]                              # the other width's image, made if the state needs it
+            for i, p, st in todo:
+                off, (lo, hi), (c0, c1) = self._offsets[i], self._blocks[i], self._chunks[i]
+                step = max(step, int(float(st['step'])))
+                for k, (full, codes, scale) in enumerate(self._KEYS):
+                    own, have = self._view(self._flat[2 + k], off, p), full in st
+                    if have == (self.state_bits == 32):       # as it is held here
+                        own.copy_(st[full] if have else byte(st[codes]))
+                        if not have:
+                            self._scales[k][lo:hi].copy_(byte(st[scale]))
+                        continue
+                    if c1 == c0:
+                        continue
+                    if other[k] is None:
+                        other[k] = torch.zeros(fp.numel(), device=fp.device, dtype=torch.float32 if have else torch.uint8)
+                    self._view(other[k], off, p).copy_(st[full] if have else byte(st[codes]))
+                    if have:
+                        call('advmix_moments_pack', P(other[k]), P(self._flat[2 + k]), P(self._scales[k]), P(self._table, c0 * 32),
+                             c1 - c0, k, st_)
+                    else:
+                        exps = torch.zeros(self._blocks[-1][1], device=fp.device, dtype=torch.uint8)
+                        exps[lo:hi].copy_(byte(st[scale]))
+                        call('advmix_moments_unpack', P(other[k]), P(exps), P(self._flat[2 + k]), P(self._table, c0 * 32),
+                             c1 - c0, k, st_)
+        self._step.fill_(step)
+        self.sync_hyper()
+
+
+def adamw_groups(model, weight_decay):
+    """Two parameter groups: what has two dimensions or more decays, the rest (biases, norm weights) does not."""
+    ps = [p for p in model.parameters() if p.requires_grad]
+    groups = [{'params': [p for p in ps if p.dim() >= 2], 'weight_decay': weight_decay},
+              {'params': [p for p in ps if p.dim() < 2], 'weight_decay': 0.0}]
+    return [g for g in groups if g['params']]
+
+
 def get_optimizer(cfg, model):
     """lib/utils/utils.py:78-94: Adam(lr) or SGD(lr, momentum, weight_decay, nesterov), both as ONE flat-buffer HIP
-    kernel per step."""
+    kernel per step; beyond the reference, ``adamw``: AdamW with TRAIN.WD on what is no bias or norm weight,
+    TRAIN.STATE_BITS (32 or 8) for its moments and TRAIN.CLIP_NORM (0: none) for the gradient's global norm."""
     if cfg.TRAIN.OPTIMIZER == 'adam':
         return FlatAdam(model.parameters(), lr=cfg.TRAIN.LR)
     if cfg.TRAIN.OPTIMIZER == 'sgd':
         return FlatSGD(model.parameters(), lr=cfg.TRAIN.LR, momentum=cfg.TRAIN.MOMENTUM,
                        weight_decay=cfg.TRAIN.WD, nesterov=cfg.TRAIN.NESTEROV)
+    if cfg.TRAIN.OPTIMIZER == 'adamw':
+        clip = float(cfg.TRAIN.get('CLIP_NORM', 0))
+        return FlatAdamW(adamw_groups(model, cfg.TRAIN.WD), lr=cfg.TRAIN.LR, state_bits=int(cfg.TRAIN.get('STATE_BITS', 32)),
+                         max_norm=clip if clip != 0 else None)
     return None
 
 

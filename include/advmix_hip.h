@@ -34,6 +34,10 @@ extern "C" {
 #define ADVMIX_ACT_RELU 1
 #define ADVMIX_ACT_LEAKY02 2   /* LeakyReLU(0.2), lib/models/Unet_generator.py:42 */
 
+#define ADVMIX_F32 0           /* activation types of the layer norm */
+#define ADVMIX_BF16 1
+#define ADVMIX_F16 2
+
 int advmix_version(void);
 /* 0 for the shipped library; non-zero bits name the measurement switches a variant build was compiled with
  * (tools/build_variant.sh, tools/variants/): such a library must never be benchmarked or shipped as the product. */
@@ -492,6 +496,48 @@ int advmix_adam(float* p, const float* g, float* m, float* v, int64_t n, const f
  * weight_decay, nesterov as 0 / 1} in device memory; buf = the momentum buffer (zero before the first step). */
 int advmix_sgd(float* p, const float* g, float* buf, int64_t n, const float* hyper, void* stream);
 int advmix_fill(float* p, float value, int64_t n, void* stream);
+
+/* ---- AdamW over the tensors of a model (torch.optim.AdamW), moments in 32 or in 8 bits; beside advmix_adam ------------
+ *   g' = g * min(1, max_norm / (|g| + 1e-6));  m' = b1 m + (1 - b1) g';  v' = b2 v + (1 - b2) g'^2
+ *   p' = p - lr wd p - lr / (1 - b1^t) * m' / (sqrt(v' / (1 - b2^t)) + eps)
+ * p, g, m, v: one flat buffer each, every tensor's start a multiple of 4 elements, the gap behind it zero.
+ * table (device): int64 [chunks][4] = {first element, elements (rounded up to 4, 1 .. 1024), group, first block of scales};
+ *   the rows of one tensor are neighbours, every row but the last 1024 elements long; rows must not overlap.
+ * hyper (device): double [1 + groups][8]; row 0 = {max_norm}, row 1 + k = {lr, b1, b2, eps, weight decay} of group k.
+ * step (device int64) is incremented by the launch (graph-replay safe).  part: NULL (no clipping, nparts 0) or what
+ *   advmix_grad_sumsq left; then the gradient's norm before clipping goes to norm_out.  coef: 4 * (8 * groups + 8) bytes of
+ *   scratch that belongs to this optimizer alone. */
+int advmix_adamw(float* p, const float* g, float* m, float* v, const int64_t* table, int chunks, const double* hyper, int groups,
+                 int64_t* step, const double* part, int nparts, float* norm_out, float* coef, void* stream);
+/* The same step on 8-bit moments: m and r = sqrt(v) as e4m3 codes, blocks of 256 elements within a tensor, each with an
+ * exponent byte E (the scale is 2^(E - 127), chosen so that the block's largest finite magnitude lies in [128, 256)).
+ * Rounded up where the fraction between two codes plus u is 1 or more: x = i * 0x9E3779B9 + key for flat element i,
+ * key = mix(t + mix(seed * 0x9E3779B9)), h = mix(x), u = (h >> 16) / 65536 for m and (h & 65535) / 65536 for r, with
+ * mix(x): x ^= x >> 15; x *= 0xBB67AE85; x ^= x >> 13 (all modulo 2^32).  r > 0 is held as no less than the smallest code; a
+ * value that is not finite is held as NaN and leaves its block's other elements alone. */
+int advmix_adamw8(float* p, const float* g, uint8_t* m, uint8_t* r, uint8_t* m_scale, uint8_t* r_scale, const int64_t* table,
+                  int chunks, const double* hyper, int groups, int64_t* step, const double* part, int nparts, float* norm_out,
+                  int seed, float* coef, void* stream);
+/* part[0 .. nparts) = partial sums of g[i]^2 in fp64, in an order that depends on n and nparts alone */
+int advmix_grad_sumsq(const float* g, int64_t n, double* part, int nparts, void* stream);
+/* fp32 moments to codes, rounded to nearest, and back; root = 1: the codes hold the square root (v and r) */
+int advmix_moments_pack(const float* x, uint8_t* codes, uint8_t* scale, const int64_t* table, int chunks, int root, void* stream);
+int advmix_moments_unpack(const uint8_t* codes, const uint8_t* scale, float* x, const int64_t* table, int chunks, int root,
+                          void* stream);
+
+/* ---- layer norm over the C channels of a row (a pixel of an NHWC map, a token); beside advmix_norm_* -------------------
+ *   y = (x - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps); fp32 statistics and parameters, activations of ``dtype``.
+ * Row r of x starts at x + r * ldx elements (dy: lddy), its channels are neighbours; y and dx are dense.  gamma / beta may be
+ * NULL (1 / 0); mean and rstd [rows] are both NULL or both written.  rows >= 1. */
+int advmix_layer_norm_fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, void* y, float* mean, float* rstd,
+                          int64_t rows, int C, int dtype, float eps, void* stream);
+/* dx, dgamma, dbeta: any of them NULL = not wanted; dgamma / dbeta are ACCUMULATED.  part (when either is wanted): scratch of
+ * advmix_layer_norm_parts(rows, C, dtype) * 2 * C floats.  The rows are summed in an order that depends on the sizes alone. */
+int advmix_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* gamma, const float* mean,
+                          const float* rstd, void* dx, float* dgamma, float* dbeta, float* part, int64_t rows, int C, int dtype,
+                          void* stream);
+/* rows of partial sums the backward pass needs (0: sizes that are not served) */
+int advmix_layer_norm_parts(int64_t rows, int C, int dtype);
 
 /* ---- three-view input pipeline on the device -------------------------------------------------
  * Replace tools/train.py:116-126 (ToTensor + Normalize), lib/dataset/advaug.py:111-170 (GridMask as

@@ -1,0 +1,379 @@
+"""ops.layer_norm on a GPU against the formula in 64 bits.
+
+Tolerances.  u = 2^-24.  A row's sums run over chains of at most n = C / 64 + 16 additions; R is the row's largest |x| over its
+sqrt(var + eps) (a row of three channels may have a standard deviation far below its mean: R is taken from the row itself).  The
+mean is off by at most n u max|x| = n u R sd, rstd by (n + 4) u relative plus what the mean's error adds, xh by e = (n (R + 2) + 8) u (1 + |xh|); y by that times
+|gamma| plus one rounding to its type.  dx = rstd (h - a - xh b): each of the three terms carries at most (n (R + 4) + 16) u of
+max|h| (1 + max|xh|)^2, times rstd, plus one rounding.  dgamma and dbeta: chains of at most N = rows / 256 + 512 additions, so
+N u times the sum of the magnitudes, plus e times sum |dy|."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}      # finfo.eps / 2
+
+
+def dev():
+    assert torch.cuda.is_available(), 'GPU tests need a GPU'
+    return torch.device('cuda:0')
+
+
+def ops():
+    from advmix_amd import ops as o
+    return o
+
+
+def rand(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed + 7 * sum(shape)))
+
+
+def rows_of(t):
+    """[rows, C] in fp64 on the CPU."""
+    t = t.detach().double().cpu()
+    return (t.permute(0, 2, 3, 1) if t.dim() == 4 else t).reshape(-1, t.shape[1] if t.dim() == 4 else t.shape[-1])
+
+
+def formula(x, gamma, beta, dy, eps):
+    x, C = rows_of(x), rows_of(x).shape[1]
+    g = torch.ones(C, dtype=torch.float64) if gamma is None else gamma.detach().double().cpu()
+    b = torch.zeros(C, dtype=torch.float64) if beta is None else beta.detach().double().cpu()
+    d = x - x.mean(1, keepdim=True)
+    rstd = ((d * d).mean(1, keepdim=True) + eps) ** -0.5
+    xh = d * rstd
+    out = {'y': xh * g + b, 'xh': xh, 'rstd': rstd, 'g': g, 'b': b, 'R': x.abs().amax(1, keepdim=True) * rstd}
+    if dy is not None:
+        dy = rows_of(dy)
+        h = dy * g
+        out.update(dx=rstd * (h - h.mean(1, keepdim=True) - xh * (h * xh).mean(1, keepdim=True)), dg=(dy * xh).sum(0),
+                   db=dy.sum(0), h=h, dy=dy)
+    return out
+
+
+def check(name, got, want, tol):
+    got = got.detach().double().cpu().reshape(want.shape)
+    bad = (got - want).abs() > tol
+    assert not bad.any(), '%s: %d of %d off, worst %.3g where %.3g is allowed' % (
+        name, int(bad.sum()), bad.numel(), float((got - want).abs()[bad].max()), float((tol + 0 * want)[bad].min()))
+
+
+def check_y(y, f):
+    C, R = f['xh'].shape[1], f['R']
+    n = C / 64 + 16
+    e = (n * (R + 2) + 8) * U * (1 + f['xh'].abs())
+    check('y', rows_of(y), f['y'], e * f['g'].abs() + 2 * U * (f['y'].abs() + f['b'].abs()) + HALF[y.dtype] * f['y'].abs() + 2.0 ** -25 * (y.dtype == torch.float16))
+
+
+def check_grads(dx, dg, db, f):
+    (rows, C), R = f['xh'].shape, f['R']
+    n = C / 64 + 16
+    if dx is not None:
+        top = f['h'].abs().amax(1, keepdim=True) * (1 + f['xh'].abs().amax(1, keepdim=True)) ** 2
+        check('dx', rows_of(dx), f['dx'], (n * (R + 4) + 16) * U * f['rstd'] * top + HALF[dx.dtype] * f['dx'].abs() + 2.0 ** -25 * (dx.dtype == torch.float16))
+    e = (n * (R + 2) + 8) * U * (1 + f['xh'].abs())
+    N = rows / 256 + 512
+    if dg is not None:
+        check('dgamma', dg, f['dg'], N * U * (f['dy'] * f['xh']).abs().sum(0) + (e * f['dy'].abs()).sum(0))
+    if db is not None:
+        check('dbeta', db, f['db'], N * U * f['dy'].abs().sum(0))
+
+
+def inputs(shape, kind, seed=0):
+    C = shape[1] if len(shape) == 4 else shape[-1]
+    x = (rand(*shape, seed=seed) + 0.5).to(dev()).to(kind)
+    dy = rand(*shape, seed=seed + 1).to(dev()).to(kind)
+    if len(shape) == 4:
+        x, dy = (t.contiguous(memory_format=torch.channels_last) for t in (x, dy))
+    return x, dy, torch.nn.Parameter((1 + 0.3 * rand(C, seed=2)).to(dev())), torch.nn.Parameter((0.3 * rand(C, seed=3)).to(dev()))
+
+
+SHAPES = [(1, 1), (5, 1), (256,), (1, 256), (3, 7), (2, 3, 33), (64, 64), (257, 100), (1537, 771), (2, 5, 768), (10, 1024),
+          (9, 1025), (33, 2048), (33, 4096), (3, 8191), (4, 16384), (3, 16385), (2, 40001), (5000, 8), (70001, 3),
+          (2, 32, 8, 6), (3, 48, 5, 7), (1, 17, 1, 1), (4, 256, 16, 12), (2, 1, 4, 4), (8, 96, 64, 48)]
+
+
+@pytest.mark.parametrize('kind', TYPES, ids=str)
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+def test_forward_and_gradients(shape, kind):
+    x, dy, gamma, beta = inputs(shape, kind)
+    x.requires_grad_()
+    y = ops().layer_norm(x, gamma, beta, eps=1e-5)
+    assert y.dtype == kind and y.shape == x.shape
+    assert y.is_contiguous(memory_format=torch.channels_last) if len(shape) == 4 else y.is_contiguous()
+    y.backward(dy)
+    f = formula(x, gamma, beta, dy, 1e-5)
+    check_y(y, f)
+    check_grads(x.grad, gamma.grad, beta.grad, f)
+    with torch.no_grad():                                   # the form that keeps no statistics gives the same bits
+        assert torch.equal(ops().layer_norm(x, gamma, beta, eps=1e-5), y)
+
+
+@pytest.mark.parametrize('kind', TYPES, ids=str)
+@pytest.mark.parametrize('how', ['gap', 'gap odd', 'offset', 'transposed', 'expanded', 'batch step', 'nchw', 'dy expanded', 'dy gap'])
+def test_layouts(how, kind):
+    """Rows that lie apart, start anywhere or are one and the same are read where they are; other layouts are copied."""
+    x, dy, gamma, beta = inputs((12, 100), kind)
+    if how == 'gap':
+        x = torch.cat([x, x], 1)[:, :100]
+    elif how == 'gap odd':
+        x = torch.cat([x, x[:, :3]], 1)[:, 2:102]
+    elif how == 'offset':
+        x = torch.cat([x.view(-1), x.view(-1)[:1]])[1:].view(12, 100)
+    elif how == 'transposed':
+        x = x.t().contiguous().t()
+    elif how == 'expanded':
+        x = x[:1].expand(12, 100)
+    elif how == 'batch step':
+        x, dy = x.view(3, 4, 100), dy.view(3, 4, 100)
+        x = torch.cat([x, x], 1)[:, 1:5]                    # rows of one distance within a batch, another between batches
+    elif how == 'nchw':
+        x, dy = x.view(3, 100, 2, 2).contiguous(), dy.view(3, 100, 2, 2).contiguous()
+    elif how == 'dy expanded':
+        dy = dy[:1, :1].expand(12, 100)
+    elif how == 'dy gap':
+        dy = torch.cat([dy, dy], 1)[:, 3:103]
+    x = x.detach().requires_grad_()
+    y = ops().layer_norm(x, gamma, beta)
+    y.backward(dy)
+    f = formula(x, gamma, beta, dy, 1e-5)
+    check_y(y, f)
+    check_grads(x.grad, gamma.grad, beta.grad, f)
+
+
+@pytest.mark.parametrize('who', ['x', 'gamma', 'beta', 'gamma beta', 'x beta', 'no gamma', 'no beta', 'neither'])
+def test_who_needs_a_gradient(who):
+    x, dy, gamma, beta = inputs((37, 200), torch.float32)
+    if who in ('no gamma', 'neither'):
+        gamma = None
+    if who in ('no beta', 'neither'):
+        beta = None
+    wants = 'x gamma beta' if who in ('no gamma', 'no beta', 'neither') else who
+    x.requires_grad_('x' in wants.split())
+    for p, name in ((gamma, 'gamma'), (beta, 'beta')):
+        if p is not None:
+            p.requires_grad_(name in wants.split())
+    y = ops().layer_norm(x, gamma, beta)
+    y.backward(dy)
+    f = formula(x, gamma, beta, dy, 1e-5)
+    check_y(y, f)
+    got = [t.grad if t is not None and t.requires_grad else None for t in (x, gamma, beta)]
+    assert all((t is None or t.grad is None) for t in (x, gamma, beta) if t is None or not t.requires_grad)
+    check_grads(*got, f)
+
+
+def test_gradients_accumulate_and_repeat_bit_for_bit():
+    x, dy, gamma, beta = inputs((3000, 96), torch.bfloat16)
+    x.requires_grad_()
+    got = []
+    for _ in range(2):
+        x.grad = gamma.grad = beta.grad = None
+        ops().layer_norm(x, gamma, beta).backward(dy)
+        got.append([t.grad.clone() for t in (x, gamma, beta)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    ops().layer_norm(x, gamma, beta).backward(dy)           # a second pass adds to what is there
+    assert torch.equal(gamma.grad, 2 * got[0][1]) and torch.equal(beta.grad, 2 * got[0][2])
+
+
+def test_mean_far_from_zero():
+    """|mean| = 1000 sd: the variance is taken around the mean, so rstd keeps its digits; the mean itself is off by n u |mean|."""
+    x, dy, gamma, beta = inputs((50, 512), torch.float32)
+    x = (x + 1000).requires_grad_()
+    y = ops().layer_norm(x, gamma, beta)
+    y.backward(dy)
+    f = formula(x, gamma, beta, dy, 1e-5)
+    check_y(y, f)
+    check_grads(x.grad, gamma.grad, beta.grad, f)
+
+
+def test_constant_rows_and_rows_that_are_not_finite():
+    x, dy, gamma, beta = inputs((8, 300), torch.float32)
+    x[1] = 3.0                                              # variance 0: y = beta
+    x[3, 5] = float('inf')
+    x[4, 299] = float('nan')
+    y = ops().layer_norm(x.requires_grad_(), gamma, beta, eps=1e-5)
+    y.sum().backward()
+    assert torch.equal(y[1], beta) and torch.isfinite(x.grad[1]).all()
+    assert torch.isnan(y[3]).any() and torch.isnan(y[4]).all() and torch.isnan(x.grad[4]).all()
+    ok = [0, 1, 2, 5, 6, 7]
+    f = formula(x[ok], gamma, beta, torch.ones(6, 300), 1e-5)
+    check_y(y[ok], f)
+    check_grads(x.grad[ok], None, None, f)
+
+
+@pytest.mark.parametrize('shape', [(0, 16), (2, 0, 16), (0, 16, 4, 4), (2, 16, 0, 4)], ids=str)
+def test_no_rows(shape):
+    x, dy, gamma, beta = inputs(shape, torch.float32)
+    y = ops().layer_norm(x.requires_grad_(), gamma, beta)
+    assert y.shape == x.shape
+    y.backward(dy)
+    assert x.grad.shape == x.shape and not gamma.grad.any() and not beta.grad.any()
+
+
+def test_gradient_against_differences():
+    """Directional derivatives of sum(w * y): central differences of the device's own fp32 forward, step 2^-6; what the third
+    derivative leaves is below 2^-12 of the slope's scale, rounding 2 C u / 2^-6 of sum |w y|."""
+    x, w, gamma, beta = inputs((20, 64), torch.float32)
+    x.requires_grad_()
+    ops().layer_norm(x, gamma, beta).backward(w)
+    for k, t in enumerate((x, gamma, beta)):
+        d = rand(*t.shape, seed=40 + k).to(dev())
+        d = d / d.norm()
+        at = [x.detach(), gamma.detach(), beta.detach()]
+        val = []
+        for s in (1, -1):
+            args = list(at)
+            args[k] = at[k] + s * 2.0 ** -6 * d
+            val.append((ops().layer_norm(*args).double() * w.double()).sum())
+        got = float((val[0] - val[1]) / 2.0 ** -5)
+        want = float((t.grad.double() * d.double()).sum())
+        tol = 2.0 ** -12 * float(t.grad.norm()) + 20 * 64 * 4 * 2 ** 6 * U
+        assert abs(got - want) <= tol, (k, got, want, tol)
+
+
+def test_group_members_that_share_parameters():
+    """Two members of one launch group, on two lanes, with the same gamma and beta: one gradient, both parts in it."""
+    o = ops()
+    x1, dy1, gamma, beta = inputs((400, 72), torch.float32)
+    x2, dy2, _, _ = inputs((4, 72, 6, 5), torch.bfloat16, seed=9)
+    x1.requires_grad_()
+    x2.requires_grad_()
+    for _ in range(2):
+        x1.grad = x2.grad = gamma.grad = beta.grad = None
+        y1, y2 = o.run_group([(o.LayerNorm, (x1, gamma, beta), 1e-5), (o.LayerNorm, (x2, gamma, beta), 1e-5)])
+        torch.autograd.backward([y1, y2], [dy1, dy2])
+        f1, f2 = formula(x1, gamma, beta, dy1, 1e-5), formula(x2, gamma, beta, dy2, 1e-5)
+        check_y(y1, f1)
+        check_y(y2, f2)
+        check_grads(x1.grad, None, None, f1)
+        check_grads(x2.grad, None, None, f2)
+        both = {k: torch.cat([f1[k], f2[k]]) for k in ('xh', 'dy', 'R')}
+        check_grads(None, gamma.grad, beta.grad, dict(both, dg=f1['dg'] + f2['dg'], db=f1['db'] + f2['db']))
+
+
+def test_between_other_ops():
+    """conv -> layer norm -> ReLU on an fp32 map, with the gradients of all of them through one backward pass."""
+    o = ops()
+    x = rand(2, 32, 8, 6).to(dev()).contiguous(memory_format=torch.channels_last).requires_grad_()
+    w = torch.nn.Parameter((0.1 * rand(64, 32, 1, 1)).to(dev()).contiguous(memory_format=torch.channels_last))
+    gamma, beta = (torch.nn.Parameter(t.to(dev())) for t in (1 + 0.3 * rand(64), 0.3 * rand(64, seed=5)))
+    dy = rand(2, 64, 8, 6, seed=3).to(dev()).contiguous(memory_format=torch.channels_last)
+    y = o.activation(o.layer_norm(o.conv2d(x, w), gamma, beta), o.ACT_RELU)
+    y.backward(dy)
+    xr, wr, gr, br = (t.detach().double().cpu().requires_grad_() for t in (x, w, gamma, beta))
+    c = torch.nn.functional.conv2d(xr, wr).permute(0, 2, 3, 1)
+    d = c - c.mean(-1, keepdim=True)
+    yr = (d / (d.square().mean(-1, keepdim=True) + 1e-5).sqrt() * gr + br).permute(0, 3, 1, 2).relu()
+    yr.backward(dy.double().cpu())
+    for a, b in ((y, yr), (x.grad, xr.grad), (w.grad, wr.grad), (gamma.grad, gr.grad), (beta.grad, br.grad)):
+        assert float((a.detach().double().cpu() - b.detach()).abs().max()) <= 1e-4 * float(b.detach().abs().max())
+
+
+def test_captured_and_replayed():
+    """Two graphs, replayed in turn with eager work of the same sizes between: each replay gives the eager bits."""
+    o = ops()
+    sets = [inputs((700, 260), torch.float16, seed=s) for s in (0, 5)]
+    want = []
+    for x, dy, gamma, beta in sets:
+        xe = x.clone().requires_grad_()
+        ye = o.layer_norm(xe, gamma, beta)
+        ye.backward(dy)
+        want.append([ye.detach().clone(), xe.grad.clone(), gamma.grad.clone(), beta.grad.clone()])
+        gamma.grad = beta.grad = None
+    graphs = []
+    for x, dy, gamma, beta in sets:
+        leaf = x.clone().requires_grad_()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            o.layer_norm(leaf, gamma, beta).backward(dy)
+        torch.cuda.current_stream().wait_stream(side)
+        leaf.grad = gamma.grad = beta.grad = None
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = o.layer_norm(leaf, gamma, beta)
+            y.backward(dy)
+        graphs.append((g, leaf, [y.detach(), leaf.grad, gamma.grad, beta.grad]))
+    for k in range(6):
+        g, leaf, out = graphs[k % 2]
+        for t in out:
+            t.fill_(float('nan')) if t is not out[2] and t is not out[3] else t.zero_()
+        g.replay()
+        if k in (1, 3):
+            x, dy, gamma, beta = sets[0]
+            o.layer_norm(x, gamma.detach(), beta.detach())
+        torch.cuda.synchronize()
+        for a, b in zip(out, want[k % 2]):
+            assert torch.equal(a, b), k
+
+
+def test_on_another_stream():
+    x, dy, gamma, beta = inputs((900, 300), torch.float32)
+    x.requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        y = ops().layer_norm(x, gamma, beta)
+        y.backward(dy)
+    torch.cuda.current_stream().wait_stream(side)
+    f = formula(x, gamma, beta, dy, 1e-5)
+    check_y(y, f)
+    check_grads(x.grad, gamma.grad, beta.grad, f)
+
+
+def test_more_than_2_31_elements():
+    """Offsets past 32 bits: 2^31 + 2^16 elements; the first and the last rows against the formula."""
+    C, rows = 512, 2 ** 22 + 128
+    x = torch.empty(rows, C, device=dev(), dtype=torch.bfloat16)
+    x.normal_(generator=torch.Generator(device=dev()).manual_seed(1))
+    gamma, beta = (torch.nn.Parameter(t.to(dev())) for t in (1 + 0.3 * rand(C), 0.3 * rand(C, seed=5)))
+    x.requires_grad_()
+    y = ops().layer_norm(x, gamma, beta)
+    dy = torch.zeros(rows, C, device=dev(), dtype=torch.bfloat16)
+    ends = torch.cat([torch.arange(40), torch.arange(rows - 200, rows)])
+    dy[ends.to(dev())] = rand(240, C, seed=11).to(dev()).bfloat16()
+    y.backward(dy)
+    f = formula(x.detach()[ends.to(dev())], gamma, beta, dy[ends.to(dev())], 1e-5)
+    check_y(y.detach()[ends.to(dev())], f)
+    dx = x.grad
+    got = dx[ends.to(dev())]
+    rows_, n = 240, C / 64 + 16
+    check_grads(got, None, None, f)
+    N = rows / 256 + 512                                    # dy is 0 elsewhere: the other rows add exact zeros
+    e = (n * (f['R'] + 2) + 8) * U * (1 + f['xh'].abs())
+    check('dgamma', gamma.grad, f['dg'], N * U * (f['dy'] * f['xh']).abs().sum(0) + (e * f['dy'].abs()).sum(0))
+    check('dbeta', beta.grad, f['db'], N * U * f['dy'].abs().sum(0))
+    assert not dx[40:rows - 200].any()
+
+
+def test_refusals_on_the_device():
+    o = ops()
+    x, dy, gamma, beta = inputs((4, 16), torch.float32)
+    with pytest.raises(TypeError):
+        o.layer_norm(x.double(), gamma, beta)
+    with pytest.raises(TypeError):
+        o.layer_norm(x, gamma.bfloat16(), beta)
+    with pytest.raises(TypeError):
+        o.layer_norm(x, gamma.cpu(), beta)
+    for bad in (gamma[:8], torch.ones(17, device=dev()), torch.ones(1, 16, device=dev()), torch.ones(32, device=dev())[::2]):
+        with pytest.raises(ValueError):
+            o.layer_norm(x, bad, beta)
+    with pytest.raises(ValueError):
+        o.layer_norm(x, gamma * 2, beta)                    # requires a gradient, is no leaf
+    with pytest.raises(ValueError):
+        o.layer_norm(x, gamma, beta, eps=-1e-5)
+    with pytest.raises(ValueError):
+        o.layer_norm(x, gamma, beta, eps=float('nan'))
+    with pytest.raises(ValueError):
+        o.layer_norm(x[:, :0])
+    with pytest.raises(ValueError):
+        o.layer_norm(x.view(1, 1, 1, 4, 16))
+    with pytest.raises(ValueError):
+        o.layer_norm(x[0, 0])
+    x.requires_grad_()
+    y = o.layer_norm(x, gamma, beta)
+    with pytest.raises(RuntimeError):                       # no second derivative
+        torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    gamma.grad = torch.zeros(32, device=dev())[::2]
+    with pytest.raises(RuntimeError):
+        o.layer_norm(x, gamma, beta).backward(dy)
