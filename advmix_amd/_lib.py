@@ -100,7 +100,7 @@ SIGNATURES = {
     'advmix_moments_pack': [_p, _p, _p, _p, _i, _i, _p],
     'advmix_moments_unpack': [_p, _p, _p, _p, _i, _i, _p],
     'advmix_layer_norm_fwd': [_p, _l, _p, _p, _p, _p, _p, _l, _i, _i, _f, _p],
-    'advmix_layer_norm_bwd': [_p, _l, _p, _l, _p, _p, _p, _p, _p, _p, _p, _l, _i, _i, _p],
+    'advmix_layer_norm_bwd': [_p, _l, _p, _l, _p, _p, _p, _p, _p, _p, _p, _i, _l, _i, _i, _p],
     'advmix_layer_norm_parts': [_l, _i, _i],
     'advmix_make_views': [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p],
     'advmix_render_targets': [_p, _p, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],

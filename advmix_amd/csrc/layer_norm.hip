@@ -5,136 +5,549 @@
 //   dgamma += sum over rows of dy * xh,  dbeta += sum over rows of dy
 // Statistics and sums are fp32; the variance is the mean of (x - mean)^2, not E[x^2] - mean^2, so that a mean far from zero
 // costs no digits.  The only rounding to fewer bits is that of y and dx to the activations' type.
+//
+// Bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  A row is held in registers by L lanes,
+// NV 16-byte chunks each, so that every pass over it after the first is free; a wave holds 64 / L short rows at once, a long
+// row is held by a workgroup of L lanes.  The backward kernel also carries its lanes' column sums of dy * xh and dy from row to
+// row - gamma's and beta's gradients cost no second reading - and leaves one partial row per workgroup; ln_fold_kernel adds
+// them in a fixed order.
 #include "common.h"
-#include <hip/hip_bf16.h>
-#include <hip/hip_fp16.h>
 
 namespace {
 
-template <typename T> __device__ __forceinline__ float ld(const T* p) { return (float)*p; }
-template <> __device__ __forceinline__ float ld<__hip_bfloat16>(const __hip_bfloat16* p) { return __bfloat162float(*p); }
-template <> __device__ __forceinline__ float ld<__half>(const __half* p) { return __half2float(*p); }
-template <typename T> __device__ __forceinline__ void sto(T* p, float v) { *p = (T)v; }
-template <> __device__ __forceinline__ void sto<__hip_bfloat16>(__hip_bfloat16* p, float v) { *p = __float2bfloat16(v); }
-template <> __device__ __forceinline__ void sto<__half>(__half* p, float v) { *p = __float2half(v); }
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float all_sum(float v) {
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+struct bf16 { uint16_t b; };
+struct f16 { _Float16 v; };
+
+// V elements of T: 16 bytes, loaded and stored at element alignment (global memory takes 16-byte accesses at any address)
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int V = 4;
+    struct __attribute__((packed, aligned(4))) Raw { u32x4 w; };
+    static __device__ __forceinline__ float get(const u32x4& w, int e) { return __uint_as_float(w[e]); }
+    static __device__ __forceinline__ u32x4 put(const float (&f)[4]) {
+        return u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    }
+    static __device__ __forceinline__ float ld(const float* p) { return *p; }
+    static __device__ __forceinline__ void st(float* p, float v) { *p = v; }
+};
+template <> struct Vec<bf16> {
+    static constexpr int V = 8;
+    struct __attribute__((packed, aligned(2))) Raw { u32x4 w; };
+    static __device__ __forceinline__ float get(const u32x4& w, int e) {
+        return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    }
+    static __device__ __forceinline__ u32x4 put(const float (&f)[8]) {
+        u32x4 w;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+        for (int k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)f[2 * k], (__bf16)f[2 * k + 1]});
+        return w;
+    }
+    static __device__ __forceinline__ float ld(const bf16* p) { return __uint_as_float((uint32_t)p->b << 16); }
+    static __device__ __forceinline__ void st(bf16* p, float v) { p->b = __builtin_bit_cast(uint16_t, (__bf16)v); }
+};
+template <> struct Vec<f16> {
+    static constexpr int V = 8;
+    struct __attribute__((packed, aligned(2))) Raw { u32x4 w; };
+    static __device__ __forceinline__ float get(const u32x4& w, int e) {
+        return (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu));
+    }
+    static __device__ __forceinline__ u32x4 put(const float (&f)[8]) {
+        u32x4 w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            w[k] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * k]) |
+                   ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)f[2 * k + 1]) << 16);
+        return w;
+    }
+    static __device__ __forceinline__ float ld(const f16* p) { return (float)p->v; }
+    static __device__ __forceinline__ void st(f16* p, float v) { p->v = (_Float16)v; }
+};
+template <typename T> __device__ __forceinline__ u32x4 load(const T* p) {
+    return reinterpret_cast<const typename Vec<T>::Raw*>(p)->w;
+}
+template <typename T> __device__ __forceinline__ void store(T* p, const u32x4& w) {
+    reinterpret_cast<typename Vec<T>::Raw*>(p)->w = w;
+}
+
+// Sum over the L neighbouring lanes of a row, in every one of them: each step adds a permutation under which the sums so far
+// are constant (lane ^ 1, lane ^ 2, mirrors of 8 and 16 lanes, the other row of 16, the other half), so no LDS is used.
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int L> __device__ __forceinline__ float lanes_sum(float v) {
+    if (L >= 2) v += dpp<0xB1>(v);
+    if (L >= 4) v += dpp<0x4E>(v);
+    if (L >= 8) v += dpp<0x141>(v);
+    if (L >= 16) v += dpp<0x140>(v);
+    if (L >= 32) {
+        const u32x2 s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    if (L >= 64) {
+        const u32x2 s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    return v;
+}
+// ... over a row held by L of the workgroup's TH lanes.  L > 64: the waves' sums meet in LDS (box: 2 * TH / 64 floats; ``flip``
+// alternates its halves, so the one barrier of a sum separates the reading of the other half from its next writing)
+template <int L, int TH> __device__ __forceinline__ float row_sum(float v, float* box, int& flip) {
+    v = lanes_sum<L < 64 ? L : 64>(v);
+    if (L > 64) {
+        constexpr int W = L / 64;
+        const int wave = threadIdx.x >> 6;
+        float* b = box + flip * (TH / 64);
+        flip ^= 1;
+        if ((threadIdx.x & 63) == 0) b[wave] = v;
+        __syncthreads();
+        v = lanes_sum<W>(b[wave / W * W + (threadIdx.x & (W - 1))]);
+    }
     return v;
 }
 
-// one wave per row
-template <typename T>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
-                                                     const float* __restrict__ beta, T* __restrict__ y, float* __restrict__ mean,
-                                                     float* __restrict__ rstd, int64_t rows, int C, float eps) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = blockIdx.x * 4ll + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4ll) {
-        const T* xr = x + r * ldx;
-        float s = 0.f;
-        for (int c = lane; c < C; c += 64) s += ld(xr + c);
-        const float mu = all_sum(s) / C;
-        float q = 0.f;
-        for (int c = lane; c < C; c += 64) { const float d = ld(xr + c) - mu; q += d * d; }
-        const float is = 1.f / sqrtf(all_sum(q) / C + eps);
-        for (int c = lane; c < C; c += 64) {
-            const float h = (ld(xr + c) - mu) * is;
-            sto(y + r * C + c, fmaf(h, gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f));
+// Where lane l of a row finds its chunk k.  With C % V != 0 the last chunk is moved back to end with the row: its elements
+// before ``from`` are another lane's (read and written twice, with the same bits; summed once).  Needs C >= V.
+template <int V, int L, bool TAIL> struct Place {
+    int at, from;
+    bool any;
+    __device__ __forceinline__ Place(int k, int l, int C) {
+        const int c = (k * L + l) * V;
+        any = c < C;
+        at = TAIL ? (c < C - V ? c : C - V) : (any ? c : 0);
+        from = any ? c - at : V;
+    }
+    __device__ __forceinline__ float only(float v, int e) const { return (TAIL ? e >= from : any) ? v : 0.f; }
+};
+
+// V elements of gamma or beta (``none`` where there is no such tensor); one uniform branch a chunk, so that all loads are in
+// flight together.
+template <int V> __device__ __forceinline__ void params(float (&to)[V], const float* __restrict__ p, int at, float none) {
+    struct __attribute__((packed, aligned(4))) Four { f32x4 v; };
+    if (p) {
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+            const f32x4 f = reinterpret_cast<const Four*>(p + at + 4 * q)->v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) to[4 * q + e] = f[e];
         }
-        if (mean && lane == 0) { mean[r] = mu; rstd[r] = is; }
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) to[e] = none;
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void ln_dx_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
-                                                    const float* __restrict__ gamma, const float* __restrict__ mean,
-                                                    const float* __restrict__ rstd, T* __restrict__ dx, int64_t rows, int C) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = blockIdx.x * 4ll + (threadIdx.x >> 6); r < rows; r += gridDim.x * 4ll) {
+constexpr int threads_of(int L) { return L > 256 ? L : 256; }
+
+template <typename T, int L, int NV, bool TAIL>
+__global__ __launch_bounds__(threads_of(L)) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
+                                                               const float* __restrict__ beta, T* __restrict__ y,
+                                                               float* __restrict__ mean, float* __restrict__ rstd, int64_t rows, int C,
+                                                               float eps) {
+    constexpr int V = Vec<T>::V, TH = threads_of(L), R = TH / L;
+    __shared__ float box[2 * TH / 64];
+    const int l = threadIdx.x % L;
+    int flip = 0;
+    const float n = (float)C;                                    // (a division: the mean of equal values is that value)
+    const int64_t step = (int64_t)gridDim.x * R;
+    int64_t r = (int64_t)blockIdx.x * R + threadIdx.x / L;
+    u32x4 next[NV];                                              // the next row is on its way while this one is worked on
+    const auto fetch = [&](int64_t row) {
+        const T* xr = x + (row < rows ? row : rows - 1) * ldx;   // (a lane without a row reads the last one)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) next[k] = load(xr + Place<V, L, TAIL>(k, l, C).at);
+    };
+    fetch(r);
+    float gm[NV][V], bt[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int at = Place<V, L, TAIL>(k, l, C).at;
+        params<V>(gm[k], gamma, at, 1.f);
+        params<V>(bt[k], beta, at, 0.f);
+    }
+    for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < rows; r0 += step, r += step) {
+        const bool in = r < rows;
+        u32x4 w[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) w[k] = next[k];
+        if (r0 + step < rows) fetch(r + step);
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const Place<V, L, TAIL> at(k, l, C);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += at.only(Vec<T>::get(w[k], e), e);
+        }
+        const float mu = row_sum<L, TH>(s, box, flip) / n;
+        float q = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const Place<V, L, TAIL> at(k, l, C);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = at.only(Vec<T>::get(w[k], e) - mu, e);
+                q = fmaf(d, d, q);
+            }
+        }
+        const float is = 1.f / sqrtf(row_sum<L, TH>(q, box, flip) / n + eps);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const Place<V, L, TAIL> at(k, l, C);
+            float o[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = fmaf((Vec<T>::get(w[k], e) - mu) * is, gm[k][e], bt[k][e]);
+            if (in && at.any) store(y + r * C + at.at, Vec<T>::put(o));
+        }
+        if (mean && in && l == 0) { mean[r] = mu; rstd[r] = is; }
+    }
+}
+
+// to[c] += v or = v
+__device__ __forceinline__ void give(float* to, int64_t c, float v, int add) {
+    if (!to) return;
+    if (add) atomicAdd(to + c, v);                               // (one per element and launch: see ln_fold_kernel)
+    else to[c] = v;
+}
+
+// part[workgroup][0][c] = sum of dy * xh, [1][c] = sum of dy over the workgroup's rows; a launch of one workgroup gives its sums
+// to dgamma and dbeta itself (part NULL).
+template <typename T, int L, int NV, bool TAIL>
+__global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
+                                                                 int64_t ldx, const float* __restrict__ gamma,
+                                                                 const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                                 T* __restrict__ dx, float* __restrict__ dgamma,
+                                                                 float* __restrict__ dbeta, float* __restrict__ part, int add,
+                                                                 int64_t rows, int C) {
+    constexpr int V = Vec<T>::V, TH = L > 512 ? L : 512, R = TH / L, W = TH / 64;
+    extern __shared__ float lds[];                               // row sums' box, then the workgroup's column sums [R waves][C]
+    const int l = threadIdx.x % L;
+    int flip = 0;
+    // 1024 lanes may have 128 registers each: with 16 elements a lane there is no room for the next row, and gamma is read again
+    // (from the L2) with every row
+    constexpr bool ROOM = L < 1024 || NV * V < 16;
+    const float n = (float)C;
+    const int64_t step = (int64_t)gridDim.x * R;
+    int64_t r = (int64_t)blockIdx.x * R + threadIdx.x / L;
+    u32x4 nw[NV], ng[NV];                                        // the next row is on its way while this one is worked on
+    float nmu, nis;
+    const auto fetch = [&](int64_t row) {
+        const int64_t rr = row < rows ? row : rows - 1;
+        const T *xr = x + rr * ldx, *gr = dy + rr * lddy;
+        nmu = mean[rr];
+        nis = rstd[rr];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int at = Place<V, L, TAIL>(k, l, C).at;
+            nw[k] = load(xr + at);
+            ng[k] = load(gr + at);
+        }
+    };
+    if (ROOM) fetch(r);
+    float gm[NV][V], dg[NV][V], db[NV][V];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) dg[k][e] = db[k][e] = 0.f;
+        if (ROOM) params<V>(gm[k], gamma, Place<V, L, TAIL>(k, l, C).at, 1.f);
+    }
+    for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < rows; r0 += step, r += step) {
+        const bool in = r < rows;
+        if (!ROOM) fetch(r);
+        const float mu = nmu, is = nis;
+        u32x4 w[NV], g[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            w[k] = nw[k];
+            g[k] = ng[k];
+        }
+        if (ROOM && r0 + step < rows) fetch(r + step);
+        float a = 0.f, b = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const Place<V, L, TAIL> at(k, l, C);
+            if (!ROOM) params<V>(gm[k], gamma, at.at, 1.f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float xh = (Vec<T>::get(w[k], e) - mu) * is;
+                const float d = in ? at.only(Vec<T>::get(g[k], e), e) : 0.f, h = d * gm[k][e];
+                const float hx = at.only(h * xh, e), dx_ = (in ? at.only(d * xh, e) : 0.f);
+                a += h;
+                b += hx;
+                dg[k][e] += dx_;
+                db[k][e] += d;
+            }
+        }
+        a = row_sum<L, TH>(a, lds, flip) / n;
+        b = row_sum<L, TH>(b, lds, flip) / n;
+        if (dx) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const Place<V, L, TAIL> at(k, l, C);
+                float o[V];
+                if (!ROOM) params<V>(gm[k], gamma, at.at, 1.f);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float xh = (Vec<T>::get(w[k], e) - mu) * is;
+                    o[e] = is * (Vec<T>::get(g[k], e) * gm[k][e] - a - xh * b);
+                }
+                if (in && at.any) store(dx + r * C + at.at, Vec<T>::put(o));
+            }
+        }
+    }
+    if (!dgamma && !dbeta) return;
+    if (R == 1) {                                                // one row at a time: a lane has its columns to itself
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const Place<V, L, TAIL> at(k, l, C);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if (!(TAIL ? e >= at.from : at.any)) continue;
+                const int c = at.at + e;
+                if (part) {
+                    part[(int64_t)blockIdx.x * 2 * C + c] = dg[k][e];
+                    part[((int64_t)blockIdx.x * 2 + 1) * C + c] = db[k][e];
+                } else {
+                    give(dgamma, c, dg[k][e], add & 1);
+                    give(dbeta, c, db[k][e], add & 2);
+                }
+            }
+        }
+        return;
+    }
+    // the rows of a wave are added across its lanes, those of different waves in LDS; first dg, then db
+    constexpr int G = R < W ? R : W;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float(&s)[NV][V] = which ? db : dg;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const Place<V, L, TAIL> at(k, l, C);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float v = s[k][e];
+#pragma unroll
+                for (int m = L; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
+                const bool mine = L >= 64 || (threadIdx.x & 63) < L;
+                if (mine && (TAIL ? e >= at.from : at.any))
+                    lds[(L >= 64 ? threadIdx.x / L : threadIdx.x >> 6) * C + at.at + e] = v;
+            }
+        }
+        __syncthreads();
+        float* to = which ? dbeta : dgamma;
+        for (int c = threadIdx.x; c < C; c += TH) {
+            float v = 0.f;
+#pragma unroll
+            for (int i = 0; i < G; ++i) v += lds[i * C + c];
+            if (part) part[((int64_t)blockIdx.x * 2 + which) * C + c] = v;
+            else give(to, c, v, add & (1 << which));
+        }
+    }
+}
+
+// The workgroups' partial sums in a fixed order: 16 columns x 64 slices of the partial rows per workgroup.  With ``add`` ONE
+// atomic addition per element, so that two launches that share a gradient lose neither's part.
+__global__ __launch_bounds__(1024) void ln_fold_kernel(const float* __restrict__ part, int parts, float* __restrict__ dgamma,
+                                                       float* __restrict__ dbeta, int add, int C) {
+    __shared__ float box[64][17];
+    const int j = threadIdx.x & 15, s = threadIdx.x >> 4;
+    const int c = blockIdx.x * 16 + j, which = blockIdx.y;
+    float v = 0.f;
+    if (c < C)
+        for (int i = s; i < parts; i += 64) v += part[((int64_t)i * 2 + which) * C + c];
+    box[s][j] = v;
+    __syncthreads();
+    if (s < 16) {                                                // 64 -> 16 -> 1
+        v = (box[s][j] + box[s + 16][j]) + (box[s + 32][j] + box[s + 48][j]);
+        box[s][j] = v;
+    }
+    __syncthreads();
+    if (s == 0 && c < C) {
+        v = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += box[i][j];
+        give(which ? dbeta : dgamma, c, v, add & (1 << which));
+    }
+}
+
+// ---- rows that no workgroup holds (or fewer channels than a chunk): a workgroup walks the row, element by element -------
+template <typename T, int TH>
+__global__ __launch_bounds__(TH) void ln_fwd_walk_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
+                                                         const float* __restrict__ beta, T* __restrict__ y, float* __restrict__ mean,
+                                                         float* __restrict__ rstd, int64_t rows, int C, float eps) {
+    __shared__ float box[2 * TH / 64];
+    int flip = 0;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const T* xr = x + r * ldx;
+        float s = 0.f, q = 0.f;
+        for (int c = threadIdx.x; c < C; c += TH) s += Vec<T>::ld(xr + c);
+        const float mu = row_sum<TH, TH>(s, box, flip) / C;
+        for (int c = threadIdx.x; c < C; c += TH) {
+            const float d = Vec<T>::ld(xr + c) - mu;
+            q = fmaf(d, d, q);
+        }
+        const float is = 1.f / sqrtf(row_sum<TH, TH>(q, box, flip) / C + eps);
+        for (int c = threadIdx.x; c < C; c += TH)
+            Vec<T>::st(y + r * C + c, fmaf((Vec<T>::ld(xr + c) - mu) * is, gamma ? gamma[c] : 1.f, beta ? beta[c] : 0.f));
+        if (mean && threadIdx.x == 0) { mean[r] = mu; rstd[r] = is; }
+    }
+}
+
+template <typename T, int TH>
+__global__ __launch_bounds__(TH) void ln_dx_walk_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
+                                                        const float* __restrict__ gamma, const float* __restrict__ mean,
+                                                        const float* __restrict__ rstd, T* __restrict__ dx, int64_t rows, int C) {
+    __shared__ float box[2 * TH / 64];
+    int flip = 0;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
         const T *xr = x + r * ldx, *gr = dy + r * lddy;
         const float mu = mean[r], is = rstd[r];
         float a = 0.f, b = 0.f;
-        for (int c = lane; c < C; c += 64) {
-            const float h = ld(gr + c) * (gamma ? gamma[c] : 1.f);
+        for (int c = threadIdx.x; c < C; c += TH) {
+            const float h = Vec<T>::ld(gr + c) * (gamma ? gamma[c] : 1.f);
             a += h;
-            b += h * ((ld(xr + c) - mu) * is);
+            b += h * ((Vec<T>::ld(xr + c) - mu) * is);
         }
-        a = all_sum(a) / C;
-        b = all_sum(b) / C;
-        for (int c = lane; c < C; c += 64) {
-            const float h = ld(gr + c) * (gamma ? gamma[c] : 1.f);
-            sto(dx + r * C + c, is * (h - a - (ld(xr + c) - mu) * is * b));
+        a = row_sum<TH, TH>(a, box, flip) / C;
+        b = row_sum<TH, TH>(b, box, flip) / C;
+        for (int c = threadIdx.x; c < C; c += TH) {
+            const float h = Vec<T>::ld(gr + c) * (gamma ? gamma[c] : 1.f);
+            Vec<T>::st(dx + r * C + c, is * (h - a - (Vec<T>::ld(xr + c) - mu) * is * b));
         }
     }
 }
 
-// part[slice][0][c] = sum of dy * xh, part[slice][1][c] = sum of dy over the slice's rows
 template <typename T>
-__global__ __launch_bounds__(256) void ln_part_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
-                                                      const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                      float* __restrict__ part, int64_t rows, int C) {
+__global__ __launch_bounds__(256) void ln_columns_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
+                                                         const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                         float* __restrict__ part, int64_t rows, int C) {
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= C) return;
     float dg = 0.f, db = 0.f;
     for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-        const float g = ld(dy + r * lddy + c);
-        dg += g * ((ld(x + r * ldx + c) - mean[r]) * rstd[r]);
+        const float g = Vec<T>::ld(dy + r * lddy + c);
+        dg = fmaf(g, (Vec<T>::ld(x + r * ldx + c) - mean[r]) * rstd[r], dg);
         db += g;
     }
     part[(blockIdx.y * 2ll) * C + c] = dg;
     part[(blockIdx.y * 2ll + 1) * C + c] = db;
 }
 
-// The slices in a fixed order; ONE atomic add per element, so that two launches that share a gradient do not lose either's part.
-__global__ __launch_bounds__(256) void ln_fold_kernel(const float* __restrict__ part, int slices, float* __restrict__ dgamma,
-                                                      float* __restrict__ dbeta, int C) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= C) return;
-    float dg = 0.f, db = 0.f;
-    for (int s = 0; s < slices; ++s) {
-        dg += part[(s * 2ll) * C + c];
-        db += part[(s * 2ll + 1) * C + c];
-    }
-    if (dgamma) atomicAdd(dgamma + c, dg);
-    if (dbeta) atomicAdd(dbeta + c, db);
+// ---- which kernel holds a row ------------------------------------------------------------------------------------------
+// chunks of 16 bytes per row -> (L lanes, NV chunks a lane); {0, 0}: no workgroup holds it
+struct Hold { int L, NV; };
+Hold hold_of(int C, int V) {
+    if (C < V) return {0, 0};
+    const int n = (C + V - 1) / V, most = V == 4 ? 4 : 2;        // at most 16 elements a lane: the backward kernel keeps five values of each
+    for (int L = 1; L <= 64; L *= 2)
+        if (n <= L) return {L, 1};
+    for (int NV = 2; NV <= most; ++NV)
+        if (n <= 64 * NV) return {64, NV};
+    for (int NV = 1; NV <= most; ++NV)
+        if (n <= 256 * NV) return {256, NV};
+    for (int NV = 1; NV <= most; NV *= 2)
+        if (n <= 1024 * NV) return {1024, NV};
+    return {0, 0};
 }
 
-int blocks_of(int64_t rows) { const int64_t n = (rows + 3) / 4; return (int)(n < 4096 ? n : 4096); }
+constexpr int MAX_PARTS = 512;
+int parts_of(int64_t rows, int C, int V) {
+    const Hold h = hold_of(C, V);
+    int64_t n;
+    if (h.L == 0) n = rows;                                      // column kernel: slices of the rows
+    else {
+        const int R = (h.L > 512 ? h.L : 512) / h.L;
+        n = (rows + R - 1) / R;
+    }
+    return (int)(n < MAX_PARTS ? n : MAX_PARTS);
+}
+
+#define HOLDS(CASE)                                                                                          \
+    CASE(1, 1) CASE(2, 1) CASE(4, 1) CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2) CASE(256, 1) \
+    CASE(256, 2) CASE(1024, 1) CASE(1024, 2)
+#define HOLDS_F32(CASE) CASE(64, 3) CASE(64, 4) CASE(256, 3) CASE(256, 4) CASE(1024, 4)
 
 template <typename T>
-int fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, void* y, float* mean, float* rstd, int64_t rows, int C,
+int fwd(const void* x_, int64_t ldx, const float* gamma, const float* beta, void* y_, float* mean, float* rstd, int64_t rows, int C,
         float eps, hipStream_t st) {
-    hipLaunchKernelGGL((ln_fwd_kernel<T>), dim3(blocks_of(rows)), dim3(256), 0, st, (const T*)x, ldx, gamma, beta, (T*)y, mean,
-                       rstd, rows, C, eps);
+    constexpr int V = Vec<T>::V;
+    const T* x = (const T*)x_;
+    T* y = (T*)y_;
+    const Hold h = hold_of(C, V);
+    const int R = h.L ? threads_of(h.L) / h.L : 1;
+    int64_t grid = (rows + R - 1) / R;
+    const int64_t cap = h.L > 256 ? 512 : 2048;                  // what 256 CUs hold at once, or twice that
+    if (grid > cap) grid = cap;
+    const dim3 g((unsigned)grid);
+#define FWD(L_, NV_)                                                                                                            \
+    if (h.L == L_ && h.NV == NV_) {                                                                                             \
+        if (C % V) hipLaunchKernelGGL((ln_fwd_kernel<T, L_, NV_, true>), g, dim3(threads_of(L_)), 0, st, x, ldx, gamma, beta, y, \
+                                      mean, rstd, rows, C, eps);                                                                \
+        else hipLaunchKernelGGL((ln_fwd_kernel<T, L_, NV_, false>), g, dim3(threads_of(L_)), 0, st, x, ldx, gamma, beta, y, mean, \
+                                rstd, rows, C, eps);                                                                            \
+    }
+    HOLDS(FWD)
+    if constexpr (V == 4) { HOLDS_F32(FWD) }
+#undef FWD
+    if (h.L == 0) {
+        if (C < V) hipLaunchKernelGGL((ln_fwd_walk_kernel<T, 64>), dim3((unsigned)(rows < 8192 ? rows : 8192)), dim3(64), 0, st, x, ldx, gamma, beta, y, mean, rstd, rows, C, eps);
+        else hipLaunchKernelGGL((ln_fwd_walk_kernel<T, 1024>), dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, x, ldx, gamma, beta, y, mean, rstd, rows, C, eps);
+    }
     ADVMIX_CHECK_LAUNCH();
     return ADVMIX_OK;
 }
 
 template <typename T>
-int bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* gamma, const float* mean, const float* rstd, void* dx,
-        float* dgamma, float* dbeta, float* part, int slices, int64_t rows, int C, hipStream_t st) {
-    if (dx)
-        hipLaunchKernelGGL((ln_dx_kernel<T>), dim3(blocks_of(rows)), dim3(256), 0, st, (const T*)dy, lddy, (const T*)x, ldx, gamma,
-                           mean, rstd, (T*)dx, rows, C);
-    if (dgamma || dbeta) {
-        hipLaunchKernelGGL((ln_part_kernel<T>), dim3(cdiv(C, 256), slices), dim3(256), 0, st, (const T*)dy, lddy, (const T*)x, ldx,
-                           mean, rstd, part, rows, C);
-        hipLaunchKernelGGL(ln_fold_kernel, dim3(cdiv(C, 256)), dim3(256), 0, st, part, slices, dgamma, dbeta, C);
+int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float* gamma, const float* mean, const float* rstd, void* dx_,
+        float* dgamma, float* dbeta, float* part, int add, int64_t rows, int C, hipStream_t st) {
+    constexpr int V = Vec<T>::V;
+    const T *x = (const T*)x_, *dy = (const T*)dy_;
+    T* dx = (T*)dx_;
+    const Hold h = hold_of(C, V);
+    const int parts = parts_of(rows, C, V);
+    const bool sums = dgamma || dbeta;
+    if (h.L) {
+        const int TH = h.L > 512 ? h.L : 512, R = TH / h.L, W = TH / 64;
+        const int64_t need = (rows + R - 1) / R;
+        const dim3 g((unsigned)(sums ? parts : (need < 2048 ? need : 2048)));
+        const size_t lds = sums && R > 1 ? sizeof(float) * ((R < W ? R : W) * (size_t)C) : 0, box = sizeof(float) * 2 * W;
+        float* pp = parts > 1 ? part : nullptr;
+#define BWD(L_, NV_)                                                                                                             \
+    if (h.L == L_ && h.NV == NV_) {                                                                                              \
+        if (C % V) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, true>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, gamma, \
+                                      mean, rstd, dx, dgamma, dbeta, pp, add, rows, C);                                          \
+        else hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, false>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, gamma, mean, \
+                                rstd, dx, dgamma, dbeta, pp, add, rows, C);                                                      \
     }
+        HOLDS(BWD)
+        if constexpr (V == 4) { HOLDS_F32(BWD) }
+#undef BWD
+        if (!sums || parts == 1) { ADVMIX_CHECK_LAUNCH(); return ADVMIX_OK; }
+    } else {
+        if (dx) {
+            if (C < V) hipLaunchKernelGGL((ln_dx_walk_kernel<T, 64>), dim3((unsigned)(rows < 8192 ? rows : 8192)), dim3(64), 0, st, dy, lddy, x, ldx, gamma, mean, rstd, dx, rows, C);
+            else hipLaunchKernelGGL((ln_dx_walk_kernel<T, 1024>), dim3((unsigned)(rows < 512 ? rows : 512)), dim3(1024), 0, st, dy, lddy, x, ldx, gamma, mean, rstd, dx, rows, C);
+        }
+        if (sums)
+            hipLaunchKernelGGL((ln_columns_kernel<T>), dim3(cdiv(C, 256), parts), dim3(256), 0, st, dy, lddy, x, ldx, mean, rstd, part, rows, C);
+    }
+    if (sums) hipLaunchKernelGGL(ln_fold_kernel, dim3(cdiv(C, 16), 2), dim3(1024), 0, st, part, parts, dgamma, dbeta, add, C);
     ADVMIX_CHECK_LAUNCH();
     return ADVMIX_OK;
 }
 
 bool sizes_ok(int64_t rows, int C, int dtype) {
-    return rows >= 1 && C >= 1 && dtype >= ADVMIX_F32 && dtype <= ADVMIX_F16 && rows <= INT64_MAX / 4 / C;
+    return rows >= 1 && C >= 1 && C <= (1 << 30) && dtype >= ADVMIX_F32 && dtype <= ADVMIX_F16 && rows <= INT64_MAX / 4 / C;
 }
 
 }  // namespace
 
 extern "C" int advmix_layer_norm_parts(int64_t rows, int C, int dtype) {
     if (!sizes_ok(rows, C, dtype)) return 0;
-    return (int)(rows < 256 ? rows : 256);
+    return parts_of(rows, C, dtype == ADVMIX_F32 ? 4 : 8);
 }
 
 extern "C" int advmix_layer_norm_fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, void* y, float* mean,
@@ -143,19 +556,18 @@ extern "C" int advmix_layer_norm_fwd(const void* x, int64_t ldx, const float* ga
         return ADVMIX_EINVAL;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == ADVMIX_F32) return fwd<float>(x, ldx, gamma, beta, y, mean, rstd, rows, C, eps, st);
-    if (dtype == ADVMIX_BF16) return fwd<__hip_bfloat16>(x, ldx, gamma, beta, y, mean, rstd, rows, C, eps, st);
-    return fwd<__half>(x, ldx, gamma, beta, y, mean, rstd, rows, C, eps, st);
+    if (dtype == ADVMIX_BF16) return fwd<bf16>(x, ldx, gamma, beta, y, mean, rstd, rows, C, eps, st);
+    return fwd<f16>(x, ldx, gamma, beta, y, mean, rstd, rows, C, eps, st);
 }
 
 extern "C" int advmix_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* gamma, const float* mean,
-                                     const float* rstd, void* dx, float* dgamma, float* dbeta, float* part, int64_t rows, int C,
+                                     const float* rstd, void* dx, float* dgamma, float* dbeta, float* part, int add, int64_t rows, int C,
                                      int dtype, void* stream) {
     if (!dy || !x || !mean || !rstd || ldx < 0 || lddy < 0 || !sizes_ok(rows, C, dtype)) return ADVMIX_EINVAL;
     if ((dgamma || dbeta) && !part) return ADVMIX_EINVAL;
+    if (!dx && !dgamma && !dbeta) return ADVMIX_OK;
     hipStream_t st = (hipStream_t)stream;
-    const int n = advmix_layer_norm_parts(rows, C, dtype);
-    if (dtype == ADVMIX_F32) return bwd<float>(dy, lddy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, part, n, rows, C, st);
-    if (dtype == ADVMIX_BF16)
-        return bwd<__hip_bfloat16>(dy, lddy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, part, n, rows, C, st);
-    return bwd<__half>(dy, lddy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, part, n, rows, C, st);
+    if (dtype == ADVMIX_F32) return bwd<float>(dy, lddy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, part, add, rows, C, st);
+    if (dtype == ADVMIX_BF16) return bwd<bf16>(dy, lddy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, part, add, rows, C, st);
+    return bwd<f16>(dy, lddy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, part, add, rows, C, st);
 }

@@ -39,7 +39,7 @@ def test_c_entries_refuse_bad_arguments():
                 dict(C=-5), dict(dtype=3), dict(dtype=-1), dict(eps=-1.0), dict(eps=float('nan')), dict(rows=2 ** 62)):
         a = dict(ok, **bad)
         assert lib.advmix_layer_norm_fwd(*[a[k] for k in ok], None) == 1, bad
-    ok = dict(dy=p, lddy=8, x=p, ldx=8, gamma=p, mean=p, rstd=p, dx=p, dg=p, db=p, part=p, rows=4, C=8, dtype=0)
+    ok = dict(dy=p, lddy=8, x=p, ldx=8, gamma=p, mean=p, rstd=p, dx=p, dg=p, db=p, part=p, add=1, rows=4, C=8, dtype=0)
     for bad in (dict(dy=None), dict(lddy=-1), dict(x=None), dict(ldx=-1), dict(mean=None), dict(rstd=None), dict(part=None), dict(rows=0),
                 dict(C=0), dict(dtype=7)):
         a = dict(ok, **bad)
