@@ -331,9 +331,19 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
                 float v = s[k][e];
 #pragma unroll
                 for (int m = L; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-                const bool mine = L >= 64 || (threadIdx.x & 63) < L;
-                if (mine && (TAIL ? e >= at.from : at.any))
-                    lds[(L >= 64 ? threadIdx.x / L : threadIdx.x >> 6) * C + at.at + e] = v;
+                s[k][e] = v;
+            }
+            const bool mine = L >= 64 || (threadIdx.x & 63) < L;
+            float* to = lds + (L >= 64 ? threadIdx.x / L : threadIdx.x >> 6) * C + at.at;
+            if (!TAIL) {                                         // C is a multiple of V: 16-byte writes
+                if (mine && at.any)
+#pragma unroll
+                    for (int q = 0; q < V; q += 4)
+                        *reinterpret_cast<f32x4*>(to + q) = f32x4{s[k][q], s[k][q + 1], s[k][q + 2], s[k][q + 3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (mine && e >= at.from) to[e] = s[k][e];
             }
         }
         __syncthreads();
@@ -348,29 +358,22 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
     }
 }
 
-// The workgroups' partial sums in a fixed order: 16 columns x 64 slices of the partial rows per workgroup.  With ``add`` ONE
+// The workgroups' partial sums in a fixed order: 32 columns x 32 slices of the partial rows per workgroup.  With ``add`` ONE
 // atomic addition per element, so that two launches that share a gradient lose neither's part.
 __global__ __launch_bounds__(1024) void ln_fold_kernel(const float* __restrict__ part, int parts, float* __restrict__ dgamma,
                                                        float* __restrict__ dbeta, int add, int C) {
-    __shared__ float box[64][17];
-    const int j = threadIdx.x & 15, s = threadIdx.x >> 4;
-    const int c = blockIdx.x * 16 + j, which = blockIdx.y;
+    __shared__ float box[32][33];
+    const int j = threadIdx.x & 31, s = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + j, which = blockIdx.y;
     float v = 0.f;
-    if (c < C)
-        for (int i = s; i < parts; i += 64) v += part[((int64_t)i * 2 + which) * C + c];
+    if (c < C) {
+#pragma unroll 8
+        for (int i = s; i < parts; i += 32) v += part[((int64_t)i * 2 + which) * C + c];
+    }
     box[s][j] = v;
     __syncthreads();
-    if (s < 16) {                                                // 64 -> 16 -> 1
-        v = (box[s][j] + box[s + 16][j]) + (box[s + 32][j] + box[s + 48][j]);
-        box[s][j] = v;
-    }
-    __syncthreads();
-    if (s == 0 && c < C) {
-        v = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v += box[i][j];
-        give(which ? dbeta : dgamma, c, v, add & (1 << which));
-    }
+    v = lanes_sum<32>(box[j][s]);                                // thread (s, j): column s, slice j
+    if (j == 0 && blockIdx.x * 32 + s < C) give(which ? dbeta : dgamma, blockIdx.x * 32 + s, v, add & (1 << which));
 }
 
 // ---- rows that no workgroup holds (or fewer channels than a chunk): a workgroup walks the row, element by element -------
@@ -453,16 +456,15 @@ Hold hold_of(int C, int V) {
     return {0, 0};
 }
 
-constexpr int MAX_PARTS = 512;
+// Workgroups of the backward kernel where it sums columns: as many as the chip holds at once (with 16 elements a lane one of
+// 512 lanes per CU, two otherwise; a long row's 1024 lanes one), each with the same number of rows, give or take one.
 int parts_of(int64_t rows, int C, int V) {
     const Hold h = hold_of(C, V);
-    int64_t n;
-    if (h.L == 0) n = rows;                                      // column kernel: slices of the rows
-    else {
-        const int R = (h.L > 512 ? h.L : 512) / h.L;
-        n = (rows + R - 1) / R;
-    }
-    return (int)(n < MAX_PARTS ? n : MAX_PARTS);
+    if (h.L == 0) return (int)(rows < 256 ? rows : 256);         // column kernel: slices of the rows
+    const int R = (h.L > 512 ? h.L : 512) / h.L;
+    const int64_t units = (rows + R - 1) / R, most = h.L == 1024 || h.NV * V >= 16 ? 256 : 512;
+    const int64_t each = (units + most - 1) / most;
+    return (int)((units + each - 1) / each);
 }
 
 #define HOLDS(CASE)                                                                                          \
@@ -534,7 +536,7 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         if (sums)
             hipLaunchKernelGGL((ln_columns_kernel<T>), dim3(cdiv(C, 256), parts), dim3(256), 0, st, dy, lddy, x, ldx, mean, rstd, part, rows, C);
     }
-    if (sums) hipLaunchKernelGGL(ln_fold_kernel, dim3(cdiv(C, 16), 2), dim3(1024), 0, st, part, parts, dgamma, dbeta, add, C);
+    if (sums) hipLaunchKernelGGL(ln_fold_kernel, dim3(cdiv(C, 32), 2), dim3(1024), 0, st, part, parts, dgamma, dbeta, add, C);
     ADVMIX_CHECK_LAUNCH();
     return ADVMIX_OK;
 }
