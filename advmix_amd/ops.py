@@ -21,7 +21,7 @@ import ctypes
 
 import torch
 
-from ._lib import call, lib
+from ._lib import call, failed, lib
 
 ACT_NONE, ACT_RELU, ACT_LEAKY = 0, 1, 2
 _CL = torch.channels_last
@@ -1170,7 +1170,11 @@ def _row_stride(t):
     """Elements between the rows of ``t`` (logical NCHW for 4-D, channels last otherwise) if its channels are neighbours and
     all its rows lie at one distance, else None."""
     if t.dim() == 4:
+        if t.is_contiguous(memory_format=_CL):
+            return t.shape[1]
         t = t.permute(0, 2, 3, 1)
+    elif t.is_contiguous():
+        return t.shape[-1]
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         return None
     step = None                                            # walk outwards: every dimension must continue the one inside it
@@ -1243,9 +1247,11 @@ class LayerNorm:
         s = torch.empty((2, rows), device=x.device, dtype=torch.float32) if stats else None
         if rows:
             at = None if s is None else s.data_ptr()
-            call('advmix_layer_norm_fwd', x.data_ptr(), _row_stride(x), None if gamma is None else gamma.data_ptr(),
-                 None if beta is None else beta.data_ptr(), y.data_ptr(), at, at and at + 4 * rows, rows, C, _LN_TYPES[x.dtype],
-                 eps, st)
+            rc = lib.advmix_layer_norm_fwd(x.data_ptr(), _row_stride(x), None if gamma is None else gamma.data_ptr(),
+                                           None if beta is None else beta.data_ptr(), y.data_ptr(), at, at and at + 4 * rows, rows,
+                                           C, _LN_TYPES[x.dtype], eps, st)
+            if rc:
+                failed('advmix_layer_norm_fwd', rc)
         return y, s
 
     @staticmethod
@@ -1282,10 +1288,13 @@ class LayerNorm:
                 if not solo:
                     keep(part)
             at = s.data_ptr()
-            call('advmix_layer_norm_bwd', dy.data_ptr(), lddy, x.data_ptr(), _row_stride(x),
-                 None if gamma is None else gamma.data_ptr(), at, at + 4 * rows, None if dx is None else dx.data_ptr(),
-                 None if dg is None else dg.data_ptr(), None if db is None else db.data_ptr(),
-                 None if part is None else part.data_ptr(), add_g + 2 * add_b, rows, C, kind, st)
+            rc = lib.advmix_layer_norm_bwd(dy.data_ptr(), lddy, x.data_ptr(), _row_stride(x),
+                                           None if gamma is None else gamma.data_ptr(), at, at + 4 * rows,
+                                           None if dx is None else dx.data_ptr(), None if dg is None else dg.data_ptr(),
+                                           None if db is None else db.data_ptr(), None if part is None else part.data_ptr(),
+                                           add_g + 2 * add_b, rows, C, kind, st)
+            if rc:
+                failed('advmix_layer_norm_bwd', rc)
         return dx, None, None
 
     @staticmethod
