@@ -27,14 +27,35 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
 }
 constexpr uint32_t GOLD = 0x9E3779B9u;      // 2^32 / golden ratio, odd
 
+// Squares in fp64: fp32 ones overflow at 1.8e19 and vanish below 1e-23.
 __global__ __launch_bounds__(256) void sumsq_kernel(const float* __restrict__ g, int64_t n, double* __restrict__ part) {
-    double s = 0.0;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) s += (double)g[i] * (double)g[i];
+    const int64_t quads = n >> 2, step = gridDim.x * 256ll;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    int64_t i = blockIdx.x * 256ll + threadIdx.x;
+    const f32x4* q = reinterpret_cast<const f32x4*>(g);
+    for (; i + 3 * step < quads; i += 4 * step) {                // four loads in flight
+        f32x4 w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = q[i + u * step];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] = fma((double)w[u][e], (double)w[u][e], s[e]);
+    }
+    for (; i < quads; i += step) {
+        const f32x4 w = q[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] = fma((double)w[e], (double)w[e], s[e]);
+    }
+    if (blockIdx.x == 0 && threadIdx.x < (n & 3)) {
+        const double w = g[4 * quads + threadIdx.x];
+        s[0] = fma(w, w, s[0]);
+    }
     __shared__ double red[4];
-    s = wave_sum_d(s);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    const double t = wave_sum_d((s[0] + s[1]) + (s[2] + s[3]));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    if (threadIdx.x == 0) part[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 __device__ double ipow(double b, int64_t t) {                    // b^t by squaring: 2 log2(t) roundings
@@ -44,16 +65,20 @@ __device__ double ipow(double b, int64_t t) {                    // b^t by squar
     return r;
 }
 
-// step += 1 and the step's coefficients per group
-__global__ void tick_kernel(const double* __restrict__ hyper, int groups, int64_t* __restrict__ step, const double* __restrict__ part,
-                            int nparts, float* __restrict__ norm_out, uint32_t seed, float* __restrict__ coef) {
+// step += 1 and the step's coefficients per group (one workgroup)
+__global__ __launch_bounds__(256) void tick_kernel(const double* __restrict__ hyper, int groups, int64_t* __restrict__ step,
+                                                   const double* __restrict__ part, int nparts, float* __restrict__ norm_out,
+                                                   uint32_t seed, float* __restrict__ coef) {
+    __shared__ double red[4];
     const int64_t t = *step + 1;
-    __syncthreads();
+    double s = 0.0;
+    for (int i = threadIdx.x; i < nparts; i += 256) s += part[i];
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();                                             // (also: everyone has read *step)
     float clip = 1.f;
     if (part) {
-        double s = 0.0;
-        for (int i = 0; i < nparts; ++i) s += part[i];
-        const double norm = sqrt(s), c = hyper[0] / (norm + 1e-6);
+        const double norm = sqrt((red[0] + red[1]) + (red[2] + red[3])), c = hyper[0] / (norm + 1e-6);
         clip = c < 1.0 || c != c ? (float)c : 1.f;
         if (threadIdx.x == 0) *norm_out = (float)norm;
     }
@@ -76,6 +101,21 @@ __global__ void tick_kernel(const double* __restrict__ hyper, int groups, int64_
     }
 }
 
+// sqrt, off by at most one place, or rounded to nearest (EXACT: the remainders of the neighbours say which it is).  The instruction
+// takes no subnormal numbers and the remainders of tiny ones vanish: below 2^-96 it works on v * 2^64.
+template <bool EXACT> __device__ __forceinline__ float root(float v) {
+    const int up = v < 0x1p-96f ? 32 : 0;
+    const float w = __builtin_amdgcn_ldexpf(v, 2 * up);
+    float s = __builtin_amdgcn_sqrtf(w);
+    if (EXACT) {
+        const float lo = __uint_as_float(__float_as_uint(s) - 1u), hi = __uint_as_float(__float_as_uint(s) + 1u);
+        const float a = fmaf(-lo, s, w), b = fmaf(-hi, s, w);
+        s = a <= 0.f ? lo : s;
+        s = b > 0.f ? hi : s;                                    // (0, infinity and NaN: both comparisons are false)
+    }
+    return __builtin_amdgcn_ldexpf(s, -up);
+}
+
 struct Coef { float lr1, b1, ob1, b2, ob2, r2, eps, lrwd; };
 
 __device__ __forceinline__ float moment1(float m, float g, const Coef& c) {
@@ -91,40 +131,65 @@ __device__ __forceinline__ float scaled(float g, float clip) {
     return g * clip;
 }
 __device__ __forceinline__ float weight(float p, float m, float r, const Coef& c) {
-    const float u = m / fmaf(r, c.r2, c.eps);
+    const float u = m * __builtin_amdgcn_rcpf(fmaf(r, c.r2, c.eps));     // (1 ulp; eps keeps it away from subnormals)
     return fmaf(-c.lr1, u, fmaf(-c.lrwd, p, p));
 }
 
+// One chunk is on its way while another is worked on; a workgroup walks the table.
 __global__ __launch_bounds__(256) void adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
-                                                    float* __restrict__ v, const Row* __restrict__ table,
+                                                    float* __restrict__ v, const Row* __restrict__ table, int chunks,
                                                     const float* __restrict__ coef, int groups) {
-    const Row row = table[blockIdx.x];
-    const int e = threadIdx.x * 4;
-    if (e >= row.count) return;
-    const int64_t i = row.first + e;
-    const Coef c = reinterpret_cast<const Coef*>(coef)[row.group];
     const float clip = coef[groups * COEF];
-    f32x4 pv = *reinterpret_cast<f32x4*>(p + i), gv = *reinterpret_cast<const f32x4*>(g + i);
-    f32x4 mv = *reinterpret_cast<f32x4*>(m + i), vv = *reinterpret_cast<f32x4*>(v + i);
+    const int e = threadIdx.x * 4;
+    Row row = table[blockIdx.x];
+    f32x4 pn, gn, mn, vn;
+    const auto fetch = [&](const Row& r) {
+        const int64_t i = r.first + (e < r.count ? e : 0);
+        pn = *reinterpret_cast<const f32x4*>(p + i);
+        gn = *reinterpret_cast<const f32x4*>(g + i);
+        mn = *reinterpret_cast<const f32x4*>(m + i);
+        vn = *reinterpret_cast<const f32x4*>(v + i);
+    };
+    fetch(row);
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const Coef k = reinterpret_cast<const Coef*>(coef)[row.group];
+        const int64_t i = row.first + e;
+        const bool in = e < row.count;
+        f32x4 pv = pn, mv = mn, vv = vn;
+        const f32x4 gv = gn;
+        if (c + (int)gridDim.x < chunks) {
+            row = table[c + gridDim.x];
+            fetch(row);
+        }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float gk = scaled(gv[k], clip);
-        mv[k] = moment1(mv[k], gk, c);
-        vv[k] = moment2(vv[k], gk, c);
-        pv[k] = weight(pv[k], mv[k], sqrtf(vv[k]), c);
+        for (int j = 0; j < 4; ++j) {
+            const float gj = scaled(gv[j], clip);
+            mv[j] = moment1(mv[j], gj, k);
+            vv[j] = moment2(vv[j], gj, k);
+            pv[j] = weight(pv[j], mv[j], root<false>(vv[j]), k);
+        }
+        if (in) {
+            *reinterpret_cast<f32x4*>(p + i) = pv;
+            *reinterpret_cast<f32x4*>(m + i) = mv;
+            *reinterpret_cast<f32x4*>(v + i) = vv;
+        }
     }
-    *reinterpret_cast<f32x4*>(p + i) = pv;
-    *reinterpret_cast<f32x4*>(m + i) = mv;
-    *reinterpret_cast<f32x4*>(v + i) = vv;
 }
 
+// Maximum over the wave, in every lane (the permutations of a butterfly: lane ^ 1, lane ^ 2, mirrors of 8 and 16, rows, halves)
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t w = __shfl_xor(v, o, 64);
-        v = w > v ? w : v;
-    }
-    return v;
+    v = max(v, dpp<0xB1>(v));
+    v = max(v, dpp<0x4E>(v));
+    v = max(v, dpp<0x141>(v));
+    v = max(v, dpp<0x140>(v));
+    u32x2 s = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(s[0], s[1]);
+    s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)max(s[0], s[1]));
 }
 __device__ __forceinline__ float pow2(int e) {                   // 2^e for -127 <= e <= 127 (2^-127 is subnormal)
     return e > -127 ? __uint_as_float((uint32_t)(e + 127) << 23) : __uint_as_float(0x00400000u);
@@ -140,97 +205,135 @@ __device__ __forceinline__ int exponent_byte(uint32_t top) {
     e = e - 7;
     return e < 0 ? 0 : e;
 }
-// e4m3 code of the magnitude z < 256 (already scaled), rounded up where fraction + u16 / 65536 >= 1
-__device__ __forceinline__ uint32_t code_of(float z, uint32_t u16) {
-    const uint32_t b = __float_as_uint(z);
-    const uint32_t big = ((b + (u16 << 4)) >> 20) - ((127 - 7) << 3);
-    const float t = z * 512.f, f = floorf(t);                    // below 2^-6: codes are 2^-9 apart
-    const uint32_t small = (uint32_t)f + (t - f >= (float)(65536u - u16) * (1.f / 65536.f) ? 1u : 0u);   // (both sides exact)
-    return z >= 0.015625f ? big : small;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ void decode(float (&x)[4], uint32_t w) {      // four e4m3 codes
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
 }
-__device__ __forceinline__ float code_value(uint32_t code) {     // magnitude of a code 0 .. 126; 127 is NaN
-    const uint32_t e = (code >> 3) & 15u, f = code & 7u;
-    const float a = e ? __uint_as_float(((e + 120u) << 23) | (f << 20)) : (float)f * (1.f / 512.f);
-    return (code & 127u) == 127u ? __uint_as_float(0x7fc00000u) : a;
+// Four codes of x * scale (below 256 in magnitude): the conversion adds the upper 20 bits of ``u`` to the fraction between two
+// codes and drops the rest, which is the rule above for u = 16 bits / 2^16, exact below the normal range too.
+__device__ __forceinline__ uint32_t encode(const float (&x)[4], float scale, const uint32_t (&u)[4]) {
+    int w = __builtin_amdgcn_cvt_sr_fp8_f32(x[0] * scale, u[0], 0, 0);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(x[1] * scale, u[1], w, 1);
+    w = __builtin_amdgcn_cvt_sr_fp8_f32(x[2] * scale, u[2], w, 2);
+    return (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(x[3] * scale, u[3], w, 3);
 }
-
-__device__ __forceinline__ uint32_t pack4(const float (&x)[4], float scale, const uint32_t (&u)[4], uint32_t least) {
-    uint32_t w = 0;
+// r > 0 is held as no less than the smallest code; only where the scaled value is below it can the code be 0
+__device__ __forceinline__ uint32_t at_least_one(uint32_t w, const float (&r)[4]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float a = fabsf(x[k]);
-        uint32_t c = code_of(a * scale, u[k]);
-        if (a > 0.f && c < least) c = least;
-        if (!(a < INFINITY)) c = 127u;
-        c |= (__float_as_uint(x[k]) >> 31) << 7;
-        w |= c << (8 * k);
-    }
+    for (int k = 0; k < 4; ++k)
+        if (r[k] > 0.f && !(w & (255u << 8 * k))) w |= 1u << 8 * k;
     return w;
+}
+// NaN for what is not finite
+__device__ __forceinline__ uint32_t poison(uint32_t w, const float (&x)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (!(fabsf(x[k]) < INFINITY)) w |= 127u << 8 * k;
+    return w;
+}
+// exponent byte of a block of 4 values a lane; not finite: out of account
+__device__ __forceinline__ int block_exponent(const float (&x)[4], bool in, bool& bad) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t = max(t, __float_as_uint(x[k]) & 0x7fffffffu);
+    t = wave_max(in ? t : 0u);
+    bad = t >= 0x7f800000u;
+    if (bad) {                                                   // (uniform, and rare)
+        t = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t = max(t, finite_bits(x[k]));
+        t = wave_max(in ? t : 0u);
+    }
+    return exponent_byte(t);
 }
 
 __global__ __launch_bounds__(256) void adamw8_kernel(float* __restrict__ p, const float* __restrict__ g, uint8_t* __restrict__ m,
                                                      uint8_t* __restrict__ r, uint8_t* __restrict__ ms, uint8_t* __restrict__ rs,
-                                                     const Row* __restrict__ table, const float* __restrict__ coef, int groups) {
-    const Row row = table[blockIdx.x];
-    const int wave = threadIdx.x >> 6;
-    if (wave * 256 >= row.count) return;                         // whole waves
-    const int e = threadIdx.x * 4;
-    const bool in = e < row.count;
-    const int64_t i = row.first + (in ? e : wave * 256);         // lanes past the end read the block's first elements
-    const int64_t blk = row.block + wave;
-    const Coef c = reinterpret_cast<const Coef*>(coef)[row.group];
+                                                     const Row* __restrict__ table, int chunks, const float* __restrict__ coef,
+                                                     int groups) {
     const float clip = coef[groups * COEF];
     const uint32_t key = reinterpret_cast<const uint32_t*>(coef)[groups * COEF + 1];
-    const float msc = pow2((int)ms[blk] - 127), rsc = pow2((int)rs[blk] - 127);
-    f32x4 pv = *reinterpret_cast<f32x4*>(p + i);
-    const f32x4 gv = *reinterpret_cast<const f32x4*>(g + i);
-    const uint32_t mw = *reinterpret_cast<const uint32_t*>(m + i), rw = *reinterpret_cast<const uint32_t*>(r + i);
-    float mv[4], rv[4];
-    uint32_t um[4], ur[4], tm = 0, tr = 0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), e = threadIdx.x * 4;
+    Row row = table[blockIdx.x];
+    f32x4 pn, gn;
+    uint32_t mn, rn;
+    int me, re;
+    const auto fetch = [&](const Row& w) {                       // lanes and waves past the end read the chunk's first elements
+        const int64_t i = w.first + (e < w.count ? e : 0);
+        pn = *reinterpret_cast<const f32x4*>(p + i);
+        gn = *reinterpret_cast<const f32x4*>(g + i);
+        mn = *reinterpret_cast<const uint32_t*>(m + i);
+        rn = *reinterpret_cast<const uint32_t*>(r + i);
+        const int64_t b = w.block + (wave * 256 < w.count ? wave : 0);
+        me = ms[b];
+        re = rs[b];
+    };
+    fetch(row);
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const Coef k = reinterpret_cast<const Coef*>(coef)[row.group];
+        const int64_t i = row.first + e, blk = row.block + wave;
+        const bool in = e < row.count, live = wave * 256 < row.count;
+        f32x4 pv = pn;
+        const f32x4 gv = gn;
+        float mv[4], rv[4];
+        decode(mv, mn);
+        decode(rv, rn);
+        const float msc = pow2(me - 127), rsc = pow2(re - 127);
+        if (c + (int)gridDim.x < chunks) {
+            row = table[c + gridDim.x];
+            fetch(row);
+        }
+        if (!live) continue;                                     // (whole waves)
+        uint32_t um[4], ur[4];
+        const uint32_t base = (uint32_t)i * GOLD + key;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t mc = mw >> (8 * k), rc = rw >> (8 * k);
-        const float a = code_value(mc & 127u) * msc, b = code_value(rc & 127u) * rsc;
-        const float gk = scaled(gv[k], clip);
-        mv[k] = moment1((mc & 128u) ? -a : a, gk, c);
-        rv[k] = sqrtf(moment2(b * b, gk, c));
-        pv[k] = weight(pv[k], mv[k], rv[k], c);
-        const uint32_t h = mix32((uint32_t)(i + k) * GOLD + key);
-        um[k] = h >> 16;
-        ur[k] = h & 0xffffu;
-        const uint32_t x = in ? finite_bits(mv[k]) : 0u, y = in ? finite_bits(rv[k]) : 0u;
-        tm = x > tm ? x : tm;
-        tr = y > tr ? y : tr;
+        for (int j = 0; j < 4; ++j) {
+            const float gj = scaled(gv[j], clip), b = rv[j] * rsc;
+            mv[j] = moment1(mv[j] * msc, gj, k);
+            rv[j] = root<true>(moment2(b * b, gj, k));
+            pv[j] = weight(pv[j], mv[j], rv[j], k);
+            const uint32_t h = mix32(base + j * GOLD);
+            um[j] = h & 0xffff0000u;
+            ur[j] = h << 16;
+        }
+        bool badm, badr;
+        const int em = block_exponent(mv, in, badm), er = block_exponent(rv, in, badr);
+        uint32_t mw = encode(mv, pow2(127 - em), um), rw = at_least_one(encode(rv, pow2(127 - er), ur), rv);
+        if (badm || badr) {
+            mw = poison(mw, mv);
+            rw = poison(rw, rv);
+        }
+        if (in) {
+            *reinterpret_cast<f32x4*>(p + i) = pv;
+            *reinterpret_cast<uint32_t*>(m + i) = mw;
+            *reinterpret_cast<uint32_t*>(r + i) = rw;
+        }
+        if ((threadIdx.x & 63) == 0) { ms[blk] = (uint8_t)em; rs[blk] = (uint8_t)er; }
     }
-    const int em = exponent_byte(wave_max(tm)), er = exponent_byte(wave_max(tr));
-    if (in) {
-        *reinterpret_cast<f32x4*>(p + i) = pv;
-        *reinterpret_cast<uint32_t*>(m + i) = pack4(mv, pow2(127 - em), um, 0u);
-        *reinterpret_cast<uint32_t*>(r + i) = pack4(rv, pow2(127 - er), ur, 1u);
-    }
-    if ((threadIdx.x & 63) == 0) { ms[blk] = (uint8_t)em; rs[blk] = (uint8_t)er; }
 }
 
 // fp32 moments <-> codes (root: the codes hold the square root); packing rounds to nearest
 __global__ __launch_bounds__(256) void pack8_kernel(const float* __restrict__ x, uint8_t* __restrict__ code, uint8_t* __restrict__ scale,
-                                                    const Row* __restrict__ table, int root) {
+                                                    const Row* __restrict__ table, int of_root) {
     const Row row = table[blockIdx.x];
     const int wave = threadIdx.x >> 6;
     if (wave * 256 >= row.count) return;
     const int e = threadIdx.x * 4;
     const bool in = e < row.count;
+    const uint32_t half[4] = {0x80000000u, 0x80000000u, 0x80000000u, 0x80000000u};
     float xv[4];
-    uint32_t top = 0, half[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const float a = in ? x[row.first + e + k] : 0.f;
-        xv[k] = root ? sqrtf(a) : a;
-        half[k] = 0x8000u;
-        const uint32_t b = finite_bits(xv[k]);
-        top = b > top ? b : top;
+        xv[k] = of_root ? root<true>(a) : a;
     }
-    const int eb = exponent_byte(wave_max(top));
-    if (in) *reinterpret_cast<uint32_t*>(code + row.first + e) = pack4(xv, pow2(127 - eb), half, root ? 1u : 0u);
+    bool bad;
+    const int eb = block_exponent(xv, in, bad);
+    uint32_t w = encode(xv, pow2(127 - eb), half);
+    if (of_root) w = at_least_one(w, xv);
+    if (bad) w = poison(w, xv);
+    if (in) *reinterpret_cast<uint32_t*>(code + row.first + e) = w;
     if ((threadIdx.x & 63) == 0) scale[row.block + wave] = (uint8_t)eb;
 }
 
@@ -240,14 +343,16 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const uint8_t* __restrict_
     const int e = threadIdx.x * 4;
     if (e >= row.count) return;
     const float s = pow2((int)scale[row.block + (threadIdx.x >> 6)] - 127);
+    float v[4];
+    decode(v, *reinterpret_cast<const uint32_t*>(code + row.first + e));
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const uint32_t c = code[row.first + e + k];
-        float a = code_value(c & 127u) * s;
-        a = root ? a * a : ((c & 128u) ? -a : a);
-        x[row.first + e + k] = a;
+        const float a = v[k] * s;
+        x[row.first + e + k] = root ? a * a : a;
     }
 }
+
+int walkers(int chunks) { return chunks < 2048 ? chunks : 2048; }        // eight workgroups per CU
 
 bool step_ok(const void* p, const void* g, const void* table, int chunks, const void* hyper, int groups, const void* step,
              const void* part, int nparts, const void* norm_out, const void* coef) {
@@ -268,8 +373,9 @@ extern "C" int advmix_adamw(float* p, const float* g, float* m, float* v, const 
                             int groups, int64_t* step, const double* part, int nparts, float* norm_out, float* coef, void* stream) {
     if (!step_ok(p, g, table, chunks, hyper, groups, step, part, nparts, norm_out, coef) || !m || !v) return ADVMIX_EINVAL;
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(tick_kernel, dim3(1), dim3(64), 0, st, hyper, groups, step, part, nparts, norm_out, 0u, coef);
-    hipLaunchKernelGGL(adamw_kernel, dim3(chunks), dim3(256), 0, st, p, g, m, v, reinterpret_cast<const Row*>(table), coef, groups);
+    hipLaunchKernelGGL(tick_kernel, dim3(1), dim3(256), 0, st, hyper, groups, step, part, nparts, norm_out, 0u, coef);
+    hipLaunchKernelGGL(adamw_kernel, dim3(walkers(chunks)), dim3(256), 0, st, p, g, m, v, reinterpret_cast<const Row*>(table), chunks,
+                       coef, groups);
     ADVMIX_CHECK_LAUNCH();
     return ADVMIX_OK;
 }
@@ -280,9 +386,9 @@ extern "C" int advmix_adamw8(float* p, const float* g, uint8_t* m, uint8_t* r, u
     if (!step_ok(p, g, table, chunks, hyper, groups, step, part, nparts, norm_out, coef) || !m || !r || !m_scale || !r_scale)
         return ADVMIX_EINVAL;
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(tick_kernel, dim3(1), dim3(64), 0, st, hyper, groups, step, part, nparts, norm_out, (uint32_t)seed, coef);
-    hipLaunchKernelGGL(adamw8_kernel, dim3(chunks), dim3(256), 0, st, p, g, m, r, m_scale, r_scale,
-                       reinterpret_cast<const Row*>(table), coef, groups);
+    hipLaunchKernelGGL(tick_kernel, dim3(1), dim3(256), 0, st, hyper, groups, step, part, nparts, norm_out, (uint32_t)seed, coef);
+    hipLaunchKernelGGL(adamw8_kernel, dim3(walkers(chunks)), dim3(256), 0, st, p, g, m, r, m_scale, r_scale,
+                       reinterpret_cast<const Row*>(table), chunks, coef, groups);
     ADVMIX_CHECK_LAUNCH();
     return ADVMIX_OK;
 }

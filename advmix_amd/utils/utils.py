@@ -302,8 +302,8 @@ class FlatAdamW(FlatAdam):
             if not (0 <= lr < float('inf') and 0 <= b1 < 1 and 0 <= b2 < 1 and 0 <= wd < float('inf')):
                 raise ValueError('FlatAdamW: lr and weight_decay must be finite and not negative, betas in [0, 1): got %r'
                                  % ((lr, b1, b2, wd),))
-            if not 1e-38 < eps < float('inf'):               # (an element that never had a gradient is 0 / eps, not 0 / 0)
-                raise ValueError('FlatAdamW: eps must be positive in fp32, got %r' % (eps,))
+            if not 1e-30 <= eps < float('inf'):              # (an element that never had a gradient is 0 / eps, not 0 / 0)
+                raise ValueError('FlatAdamW: eps must be at least 1e-30, got %r' % (eps,))
             rows += [lr, float(b1), float(b2), eps, wd] + [0.0] * (self.HYPER - 5)
         return tuple(rows)
 
