@@ -135,45 +135,42 @@ __device__ __forceinline__ float weight(float p, float m, float r, const Coef& c
     return fmaf(-c.lr1, u, fmaf(-c.lrwd, p, p));
 }
 
-// One chunk is on its way while another is worked on; a workgroup walks the table.
+// NT: the step's data is larger than the last-level cache (256 MB), so it goes past the caches in both directions; see stream_past.
+template <bool NT, typename T> __device__ __forceinline__ T ldv(const T* p) {
+    return NT ? __builtin_nontemporal_load(p) : *p;
+}
+template <bool NT, typename T> __device__ __forceinline__ void stv(T* p, T v) {
+    if (NT) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+__device__ __forceinline__ const f32x4* quad(const float* p) { return reinterpret_cast<const f32x4*>(p); }
+__device__ __forceinline__ f32x4* quad(float* p) { return reinterpret_cast<f32x4*>(p); }
+
+// Bound by memory: 28 bytes an element.  A workgroup takes one chunk and ends (walking workgroups with the next chunk on its way
+// are slower: 28.5 M elements 170 us with 2048 of them, 155 us this way).
+template <bool NT>
 __global__ __launch_bounds__(256) void adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
-                                                    float* __restrict__ v, const Row* __restrict__ table, int chunks,
+                                                    float* __restrict__ v, const Row* __restrict__ table,
                                                     const float* __restrict__ coef, int groups) {
-    const float clip = coef[groups * COEF];
+    const Row row = table[blockIdx.x];
     const int e = threadIdx.x * 4;
-    Row row = table[blockIdx.x];
-    f32x4 pn, gn, mn, vn;
-    const auto fetch = [&](const Row& r) {
-        const int64_t i = r.first + (e < r.count ? e : 0);
-        pn = *reinterpret_cast<const f32x4*>(p + i);
-        gn = *reinterpret_cast<const f32x4*>(g + i);
-        mn = *reinterpret_cast<const f32x4*>(m + i);
-        vn = *reinterpret_cast<const f32x4*>(v + i);
-    };
-    fetch(row);
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const Coef k = reinterpret_cast<const Coef*>(coef)[row.group];
-        const int64_t i = row.first + e;
-        const bool in = e < row.count;
-        f32x4 pv = pn, mv = mn, vv = vn;
-        const f32x4 gv = gn;
-        if (c + (int)gridDim.x < chunks) {
-            row = table[c + gridDim.x];
-            fetch(row);
-        }
+    if (e >= row.count) return;
+    const int64_t i = row.first + e;
+    f32x4 pv = ldv<NT>(quad(p + i));
+    const f32x4 gv = ldv<NT>(quad(g + i));
+    f32x4 mv = ldv<NT>(quad(m + i)), vv = ldv<NT>(quad(v + i));
+    const Coef k = reinterpret_cast<const Coef*>(coef)[row.group];
+    const float clip = coef[groups * COEF];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float gj = scaled(gv[j], clip);
-            mv[j] = moment1(mv[j], gj, k);
-            vv[j] = moment2(vv[j], gj, k);
-            pv[j] = weight(pv[j], mv[j], root<false>(vv[j]), k);
-        }
-        if (in) {
-            *reinterpret_cast<f32x4*>(p + i) = pv;
-            *reinterpret_cast<f32x4*>(m + i) = mv;
-            *reinterpret_cast<f32x4*>(v + i) = vv;
-        }
+    for (int j = 0; j < 4; ++j) {
+        const float gj = scaled(gv[j], clip);
+        mv[j] = moment1(mv[j], gj, k);
+        vv[j] = moment2(vv[j], gj, k);
+        pv[j] = weight(pv[j], mv[j], root<false>(vv[j]), k);
     }
+    stv<NT>(quad(p + i), pv);
+    stv<NT>(quad(m + i), mv);
+    stv<NT>(quad(v + i), vv);
 }
 
 // Maximum over the wave, in every lane (the permutations of a butterfly: lane ^ 1, lane ^ 2, mirrors of 8 and 16, rows, halves)
@@ -248,69 +245,51 @@ __device__ __forceinline__ int block_exponent(const float (&x)[4], bool in, bool
     return exponent_byte(t);
 }
 
+// 16 bytes an element and some 90 instructions: close to where the vector units would bound it, hence the conversion instructions,
+// the roots off one instruction and maxima without LDS (146 instructions an element and 103 us for 28.5 M elements without them).
+template <bool NT>
 __global__ __launch_bounds__(256) void adamw8_kernel(float* __restrict__ p, const float* __restrict__ g, uint8_t* __restrict__ m,
                                                      uint8_t* __restrict__ r, uint8_t* __restrict__ ms, uint8_t* __restrict__ rs,
-                                                     const Row* __restrict__ table, int chunks, const float* __restrict__ coef,
-                                                     int groups) {
-    const float clip = coef[groups * COEF];
-    const uint32_t key = reinterpret_cast<const uint32_t*>(coef)[groups * COEF + 1];
+                                                     const Row* __restrict__ table, const float* __restrict__ coef, int groups) {
+    const Row row = table[blockIdx.x];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), e = threadIdx.x * 4;
-    Row row = table[blockIdx.x];
-    f32x4 pn, gn;
-    uint32_t mn, rn;
-    int me, re;
-    const auto fetch = [&](const Row& w) {                       // lanes and waves past the end read the chunk's first elements
-        const int64_t i = w.first + (e < w.count ? e : 0);
-        pn = *reinterpret_cast<const f32x4*>(p + i);
-        gn = *reinterpret_cast<const f32x4*>(g + i);
-        mn = *reinterpret_cast<const uint32_t*>(m + i);
-        rn = *reinterpret_cast<const uint32_t*>(r + i);
-        const int64_t b = w.block + (wave * 256 < w.count ? wave : 0);
-        me = ms[b];
-        re = rs[b];
-    };
-    fetch(row);
-    for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-        const Coef k = reinterpret_cast<const Coef*>(coef)[row.group];
-        const int64_t i = row.first + e, blk = row.block + wave;
-        const bool in = e < row.count, live = wave * 256 < row.count;
-        f32x4 pv = pn;
-        const f32x4 gv = gn;
-        float mv[4], rv[4];
-        decode(mv, mn);
-        decode(rv, rn);
-        const float msc = pow2(me - 127), rsc = pow2(re - 127);
-        if (c + (int)gridDim.x < chunks) {
-            row = table[c + gridDim.x];
-            fetch(row);
-        }
-        if (!live) continue;                                     // (whole waves)
-        uint32_t um[4], ur[4];
-        const uint32_t base = (uint32_t)i * GOLD + key;
+    if (wave * 256 >= row.count) return;                         // (whole waves)
+    const bool in = e < row.count;
+    const int64_t i = row.first + (in ? e : wave * 256), blk = row.block + wave;      // lanes past the end read the block's first elements
+    f32x4 pv = ldv<NT>(quad(p + i));
+    const f32x4 gv = ldv<NT>(quad(g + i));
+    const uint32_t mc = ldv<NT>(reinterpret_cast<const uint32_t*>(m + i)), rc = ldv<NT>(reinterpret_cast<const uint32_t*>(r + i));
+    const float msc = pow2((int)ms[blk] - 127), rsc = pow2((int)rs[blk] - 127);
+    const Coef k = reinterpret_cast<const Coef*>(coef)[row.group];
+    const float clip = coef[groups * COEF];
+    const uint32_t base = (uint32_t)i * GOLD + reinterpret_cast<const uint32_t*>(coef)[groups * COEF + 1];
+    float mv[4], rv[4];
+    uint32_t um[4], ur[4];
+    decode(mv, mc);
+    decode(rv, rc);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float gj = scaled(gv[j], clip), b = rv[j] * rsc;
-            mv[j] = moment1(mv[j] * msc, gj, k);
-            rv[j] = root<true>(moment2(b * b, gj, k));
-            pv[j] = weight(pv[j], mv[j], rv[j], k);
-            const uint32_t h = mix32(base + j * GOLD);
-            um[j] = h & 0xffff0000u;
-            ur[j] = h << 16;
-        }
-        bool badm, badr;
-        const int em = block_exponent(mv, in, badm), er = block_exponent(rv, in, badr);
-        uint32_t mw = encode(mv, pow2(127 - em), um), rw = at_least_one(encode(rv, pow2(127 - er), ur), rv);
-        if (badm || badr) {
-            mw = poison(mw, mv);
-            rw = poison(rw, rv);
-        }
-        if (in) {
-            *reinterpret_cast<f32x4*>(p + i) = pv;
-            *reinterpret_cast<uint32_t*>(m + i) = mw;
-            *reinterpret_cast<uint32_t*>(r + i) = rw;
-        }
-        if ((threadIdx.x & 63) == 0) { ms[blk] = (uint8_t)em; rs[blk] = (uint8_t)er; }
+    for (int j = 0; j < 4; ++j) {
+        const float gj = scaled(gv[j], clip), b = rv[j] * rsc;
+        mv[j] = moment1(mv[j] * msc, gj, k);
+        rv[j] = root<true>(moment2(b * b, gj, k));
+        pv[j] = weight(pv[j], mv[j], rv[j], k);
+        const uint32_t h = mix32(base + j * GOLD);
+        um[j] = h & 0xffff0000u;
+        ur[j] = h << 16;
     }
+    bool badm, badr;
+    const int em = block_exponent(mv, in, badm), er = block_exponent(rv, in, badr);
+    uint32_t mw = encode(mv, pow2(127 - em), um), rw = at_least_one(encode(rv, pow2(127 - er), ur), rv);
+    if (badm || badr) {
+        mw = poison(mw, mv);
+        rw = poison(rw, rv);
+    }
+    if (in) {
+        stv<NT>(quad(p + i), pv);
+        stv<NT>(reinterpret_cast<uint32_t*>(m + i), mw);
+        stv<NT>(reinterpret_cast<uint32_t*>(r + i), rw);
+    }
+    if ((threadIdx.x & 63) == 0) { ms[blk] = (uint8_t)em; rs[blk] = (uint8_t)er; }
 }
 
 // fp32 moments <-> codes (root: the codes hold the square root); packing rounds to nearest
@@ -352,7 +331,10 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const uint8_t* __restrict_
     }
 }
 
-int walkers(int chunks) { return chunks < 2048 ? chunks : 2048; }        // eight workgroups per CU
+// What a step touches, from its chunks, against the last-level cache of 256 MB.  Past the caches / through them, us: 63.6 M elements
+// in 32 bits (1.8 GB, clipped) 320 / 396, 28.5 M (800 MB) 138 / 152, 10 M (280 MB) 50 / 57, 3 M (84 MB) 18.8 / 17.4; in 8 bits 28.5 M
+// (456 MB) 85.6 / 89.2, 10 M (160 MB) 33.6 / 33.2.
+bool stream_past(int chunks, int bytes) { return (int64_t)chunks * 1024 * bytes > (256ll << 20); }
 
 bool step_ok(const void* p, const void* g, const void* table, int chunks, const void* hyper, int groups, const void* step,
              const void* part, int nparts, const void* norm_out, const void* coef) {
@@ -374,8 +356,9 @@ extern "C" int advmix_adamw(float* p, const float* g, float* m, float* v, const 
     if (!step_ok(p, g, table, chunks, hyper, groups, step, part, nparts, norm_out, coef) || !m || !v) return ADVMIX_EINVAL;
     hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(tick_kernel, dim3(1), dim3(256), 0, st, hyper, groups, step, part, nparts, norm_out, 0u, coef);
-    hipLaunchKernelGGL(adamw_kernel, dim3(walkers(chunks)), dim3(256), 0, st, p, g, m, v, reinterpret_cast<const Row*>(table), chunks,
-                       coef, groups);
+    const Row* rows = reinterpret_cast<const Row*>(table);
+    if (stream_past(chunks, 28)) hipLaunchKernelGGL(adamw_kernel<true>, dim3(chunks), dim3(256), 0, st, p, g, m, v, rows, coef, groups);
+    else hipLaunchKernelGGL(adamw_kernel<false>, dim3(chunks), dim3(256), 0, st, p, g, m, v, rows, coef, groups);
     ADVMIX_CHECK_LAUNCH();
     return ADVMIX_OK;
 }
@@ -387,8 +370,10 @@ extern "C" int advmix_adamw8(float* p, const float* g, uint8_t* m, uint8_t* r, u
         return ADVMIX_EINVAL;
     hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(tick_kernel, dim3(1), dim3(256), 0, st, hyper, groups, step, part, nparts, norm_out, (uint32_t)seed, coef);
-    hipLaunchKernelGGL(adamw8_kernel, dim3(walkers(chunks)), dim3(256), 0, st, p, g, m, r, m_scale, r_scale,
-                       reinterpret_cast<const Row*>(table), chunks, coef, groups);
+    const Row* rows = reinterpret_cast<const Row*>(table);
+    if (stream_past(chunks, 16))
+        hipLaunchKernelGGL(adamw8_kernel<true>, dim3(chunks), dim3(256), 0, st, p, g, m, r, m_scale, r_scale, rows, coef, groups);
+    else hipLaunchKernelGGL(adamw8_kernel<false>, dim3(chunks), dim3(256), 0, st, p, g, m, r, m_scale, r_scale, rows, coef, groups);
     ADVMIX_CHECK_LAUNCH();
     return ADVMIX_OK;
 }

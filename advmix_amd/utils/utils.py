@@ -2,6 +2,7 @@
 lr only) backed by ONE flat-buffer HIP Adam kernel instead of 878 per-tensor launches, and
 ``save_checkpoint`` (:97-108)."""
 import ctypes
+import operator
 import os
 
 import torch
@@ -331,22 +332,44 @@ class FlatAdamW(FlatAdam):
         if self.state_bits == 8:
             self._flat = self._flat[:2] + tuple(torch.zeros(fp.numel(), device=dev, dtype=torch.uint8) for _ in range(2))
             self._scales = tuple(torch.zeros(block, device=dev, dtype=torch.uint8) for _ in range(2))
+        self._index, self._ps, self._raw_host = dev.index, self._params(), self._hyper_raw()
+        fp, fg, m, v = self._flat                             # (these buffers live as long as the optimizer)
+        P = lambda t: None if t is None else t.data_ptr()          # noqa: E731
+        rest = (P(self._table), len(rows), P(self._hyper), len(self.param_groups), P(self._step), P(self._parts),
+                self.PARTS if self._clips else 0, P(self.grad_norm))
+        if self.state_bits == 8:
+            self._step_args = ('advmix_adamw8', P(fp), P(fg), P(m), P(v), *map(P, self._scales), *rest, self.seed, P(self._coef))
+        else:
+            self._step_args = ('advmix_adamw', P(fp), P(fg), P(m), P(v), *rest, P(self._coef))
+        self._norm_args = (P(fg), fg.numel(), P(self._parts), self.PARTS)
 
     def flat_state(self):
         """[parameters, m, v, step]; with 8 bits [parameters, m codes, r codes, step, m exponent bytes, r exponent bytes]."""
         return super().flat_state() + (list(self._scales) if self.state_bits == 8 else [])
 
+    def _hyper_raw(self):
+        return [self.max_norm] + [x for g in self.param_groups for x in (
+            float(g['lr']), g['betas'], g['eps'], g['weight_decay'], g.get('amsgrad'), g.get('maximize'))]
+
     def sync_hyper(self):
         self._ensure_flat()
+        raw = self._hyper_raw()
+        if raw == self._raw_host:                             # (nothing to check or to send)
+            return
         cur = self._hyper_tuple()
         if cur != self._hyper_host:
             self._hyper.copy_(torch.tensor(cur, dtype=torch.float64))
             self._hyper_host = cur
+        self._raw_host = raw
 
     def zero_grad(self, set_to_none=False):
         self._ensure_flat()
         with torch.cuda.device(self._flat[0].device):
             super().zero_grad(set_to_none)
+
+    def _attach_grads(self, strict):
+        if not all(map(operator.is_, [p.grad for p in self._ps], self._grad_views)):      # (a step of 300 tensors: 10 us of this)
+            super()._attach_grads(strict)
 
     @torch.no_grad()
     def step(self, closure=None, sync_hyper=True):
@@ -356,19 +379,17 @@ class FlatAdamW(FlatAdam):
         if sync_hyper and not torch.cuda.is_current_stream_capturing():
             self.sync_hyper()
         self._attach_grads(strict=True)
-        fp, fg, m, v = self._flat
-        P = lambda t: None if t is None else ctypes.c_void_p(t.data_ptr())       # noqa: E731
-        with torch.cuda.device(fp.device):
-            st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-            if self._clips:
-                call('advmix_grad_sumsq', P(fg), fg.numel(), P(self._parts), self.PARTS, st)
-            rest = (P(self._table), len(self._table), P(self._hyper), len(self.param_groups), P(self._step), P(self._parts),
-                    self.PARTS if self._clips else 0, P(self.grad_norm))
-            if self.state_bits == 8:
-                call('advmix_adamw8', P(fp), P(fg), P(m), P(v), P(self._scales[0]), P(self._scales[1]), *rest, self.seed,
-                     P(self._coef), st)
-            else:
-                call('advmix_adamw', P(fp), P(fg), P(m), P(v), *rest, P(self._coef), st)
+        index = self._index
+        if index != torch.cuda.current_device():
+            with torch.cuda.device(index):
+                return self._launch(index)
+        self._launch(index)
+
+    def _launch(self, index):
+        st = torch.cuda.current_stream(index).cuda_stream
+        if self._clips:
+            call('advmix_grad_sumsq', *self._norm_args, st)
+        call(*self._step_args, st)
 
     # ---- state ------------------------------------------------------------------------------
     _KEYS = (('exp_avg', 'exp_avg_codes', 'exp_avg_scale'), ('exp_avg_sq', 'exp_avg_root_codes', 'exp_avg_root_scale'))
