@@ -26,7 +26,7 @@ struct f16 { _Float16 v; };
 template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr int V = 4;
-    struct __attribute__((packed, aligned(4))) Raw { u32x4 w; };
+    typedef u32x4 Raw __attribute__((aligned(4)));
     static __device__ __forceinline__ float get(const u32x4& w, int e) { return __uint_as_float(w[e]); }
     static __device__ __forceinline__ u32x4 put(const float (&f)[4]) {
         return u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
@@ -36,7 +36,7 @@ template <> struct Vec<float> {
 };
 template <> struct Vec<bf16> {
     static constexpr int V = 8;
-    struct __attribute__((packed, aligned(2))) Raw { u32x4 w; };
+    typedef u32x4 Raw __attribute__((aligned(2)));
     static __device__ __forceinline__ float get(const u32x4& w, int e) {
         return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
     }
@@ -51,7 +51,7 @@ template <> struct Vec<bf16> {
 };
 template <> struct Vec<f16> {
     static constexpr int V = 8;
-    struct __attribute__((packed, aligned(2))) Raw { u32x4 w; };
+    typedef u32x4 Raw __attribute__((aligned(2)));
     static __device__ __forceinline__ float get(const u32x4& w, int e) {
         return (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu));
     }
@@ -67,10 +67,13 @@ template <> struct Vec<f16> {
     static __device__ __forceinline__ void st(f16* p, float v) { p->v = (_Float16)v; }
 };
 template <typename T> __device__ __forceinline__ u32x4 load(const T* p) {
-    return reinterpret_cast<const typename Vec<T>::Raw*>(p)->w;
+    return *reinterpret_cast<const typename Vec<T>::Raw*>(p);
+}
+template <typename T> __device__ __forceinline__ u32x4 load_past(const T* p) {            // past the caches
+    return __builtin_nontemporal_load(reinterpret_cast<const typename Vec<T>::Raw*>(p));
 }
 template <typename T> __device__ __forceinline__ void store(T* p, const u32x4& w) {
-    reinterpret_cast<typename Vec<T>::Raw*>(p)->w = w;
+    *reinterpret_cast<typename Vec<T>::Raw*>(p) = w;
 }
 
 // Sum over the L neighbouring lanes of a row, in every one of them: each step adds a permutation under which the sums so far
@@ -126,11 +129,11 @@ template <int V, int L, bool TAIL> struct Place {
 // V elements of gamma or beta (``none`` where there is no such tensor); one uniform branch a chunk, so that all loads are in
 // flight together.
 template <int V> __device__ __forceinline__ void params(float (&to)[V], const float* __restrict__ p, int at, float none) {
-    struct __attribute__((packed, aligned(4))) Four { f32x4 v; };
+    typedef f32x4 Four __attribute__((aligned(4)));
     if (p) {
 #pragma unroll
         for (int q = 0; q < V / 4; ++q) {
-            const f32x4 f = reinterpret_cast<const Four*>(p + at + 4 * q)->v;
+            const f32x4 f = *reinterpret_cast<const Four*>(p + at + 4 * q);
 #pragma unroll
             for (int e = 0; e < 4; ++e) to[4 * q + e] = f[e];
         }
@@ -214,7 +217,8 @@ __device__ __forceinline__ void give(float* to, int64_t c, float v, int add) {
 
 // part[workgroup][0][c] = sum of dy * xh, [1][c] = sum of dy over the workgroup's rows; a launch of one workgroup gives its sums
 // to dgamma and dbeta itself (part NULL).
-template <typename T, int L, int NV, bool TAIL>
+// PAST: x and dy are read past the caches (both are dead after this kernel).
+template <typename T, int L, int NV, bool TAIL, bool PAST>
 __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
                                                                  int64_t ldx, const float* __restrict__ gamma,
                                                                  const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -241,8 +245,8 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int at = Place<V, L, TAIL>(k, l, C).at;
-            nw[k] = load(xr + at);
-            ng[k] = load(gr + at);
+            nw[k] = PAST ? load_past(xr + at) : load(xr + at);
+            ng[k] = PAST ? load_past(gr + at) : load(gr + at);
         }
     };
     if (ROOM) fetch(r);
@@ -517,12 +521,18 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         const dim3 g((unsigned)(sums ? parts : (need < 2048 ? need : 2048)));
         const size_t lds = sums && R > 1 ? sizeof(float) * ((R < W ? R : W) * (size_t)C) : 0, box = sizeof(float) * 2 * W;
         float* pp = parts > 1 ? part : nullptr;
+        // x, dy and dx against the last-level cache of 256 MB; read past the caches / through them, us: 30000 x 1024 fp32 (369 MB)
+        // 63 / 73, 100000 x 256 fp32 (307 MB) 55 / 58, 16384 x 4096 bf16 (403 MB) 75 / 77; 6144 x 768 bf16 (28 MB) 11.8 / 11.4.
+        // (Odd widths keep to the caches, where neighbouring rows share lines.)
+        const bool past = rows * C * (int64_t)sizeof(T) * 3 > (256ll << 20);
 #define BWD(L_, NV_)                                                                                                             \
     if (h.L == L_ && h.NV == NV_) {                                                                                              \
-        if (C % V) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, true>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, gamma, \
+        if (C % V) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, true, false>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, gamma, \
                                       mean, rstd, dx, dgamma, dbeta, pp, add, rows, C);                                          \
-        else hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, false>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, gamma, mean, \
-                                rstd, dx, dgamma, dbeta, pp, add, rows, C);                                                      \
+        else if (past) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, false, true>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, \
+                                          ldx, gamma, mean, rstd, dx, dgamma, dbeta, pp, add, rows, C);                          \
+        else hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, false, false>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, \
+                                gamma, mean, rstd, dx, dgamma, dbeta, pp, add, rows, C);                                         \
     }
         HOLDS(BWD)
         if constexpr (V == 4) { HOLDS_F32(BWD) }
