@@ -96,6 +96,23 @@ template <int L> __device__ __forceinline__ float lanes_sum(float v) {
     }
     return v;
 }
+// Sum over the lanes of a wave with the same place in their rows of L lanes, in every one of them (rotations within 16 lanes
+// first: what they add has a period by then).
+template <int L> __device__ __forceinline__ float places_sum(float v) {
+    if (L <= 8) v += dpp<0x128>(v);
+    if (L <= 4) v += dpp<0x124>(v);
+    if (L <= 2) v += dpp<0x122>(v);
+    if (L <= 1) v += dpp<0x121>(v);
+    if (L <= 16) {
+        const u32x2 s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    if (L <= 32) {
+        const u32x2 s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    return v;
+}
 // ... over a row held by L of the workgroup's TH lanes.  L > 64: the waves' sums meet in LDS (box: 2 * TH / 64 floats; ``flip``
 // alternates its halves, so the one barrier of a sum separates the reading of the other half from its next writing)
 template <int L, int TH> __device__ __forceinline__ float row_sum(float v, float* box, int& flip) {
@@ -323,61 +340,69 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
     }
     // the rows of a wave are added across its lanes, those of different waves in LDS; first dg, then db
     constexpr int G = R < W ? R : W;
-#pragma unroll
+    const int wide = TAIL ? C + (C >> 3) + 1 : C;                // (element by element, every ninth word is left out: a lane's next
+#pragma unroll                                                   //  eight columns then start in another bank)
     for (int which = 0; which < 2; ++which) {
-        float(&s)[NV][V] = which ? db : dg;
+        const float(&s)[NV][V] = which ? db : dg;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const Place<V, L, TAIL> at(k, l, C);
+            float v[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float v = s[k][e];
-#pragma unroll
-                for (int m = L; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
-                s[k][e] = v;
-            }
+            for (int e = 0; e < V; ++e) v[e] = places_sum<L>(s[k][e]);
             const bool mine = L >= 64 || (threadIdx.x & 63) < L;
-            float* to = lds + (L >= 64 ? threadIdx.x / L : threadIdx.x >> 6) * C + at.at;
+            float* to = lds + (L >= 64 ? threadIdx.x / L : threadIdx.x >> 6) * wide;
             if (!TAIL) {                                         // C is a multiple of V: 16-byte writes
                 if (mine && at.any)
 #pragma unroll
                     for (int q = 0; q < V; q += 4)
-                        *reinterpret_cast<f32x4*>(to + q) = f32x4{s[k][q], s[k][q + 1], s[k][q + 2], s[k][q + 3]};
+                        *reinterpret_cast<f32x4*>(to + at.at + q) = f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
             } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e)
-                    if (mine && e >= at.from) to[e] = s[k][e];
+                for (int e = 0; e < V; ++e) {
+                    const int c = at.at + e;
+                    if (mine && e >= at.from) to[c + (c >> 3)] = v[e];
+                }
             }
         }
         __syncthreads();
         float* to = which ? dbeta : dgamma;
         for (int c = threadIdx.x; c < C; c += TH) {
+            const int j = TAIL ? c + (c >> 3) : c;
             float v = 0.f;
 #pragma unroll
-            for (int i = 0; i < G; ++i) v += lds[i * C + c];
+            for (int i = 0; i < G; ++i) v += lds[i * wide + j];
             if (part) part[((int64_t)blockIdx.x * 2 + which) * C + c] = v;
             else give(to, c, v, add & (1 << which));
         }
     }
 }
 
-// The workgroups' partial sums in a fixed order: 32 columns x 32 slices of the partial rows per workgroup.  With ``add`` ONE
-// atomic addition per element, so that two launches that share a gradient lose neither's part.
+// The workgroups' partial sums in a fixed order: 16 columns x 64 slices of the partial rows per workgroup, so that a thread has at
+// most eight loads, all in flight.  With ``add`` ONE atomic addition per element, so that two launches that share a gradient lose
+// neither's part.
+constexpr int FOLD = 16;
 __global__ __launch_bounds__(1024) void ln_fold_kernel(const float* __restrict__ part, int parts, float* __restrict__ dgamma,
                                                        float* __restrict__ dbeta, int add, int C) {
-    __shared__ float box[32][33];
-    const int j = threadIdx.x & 31, s = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + j, which = blockIdx.y;
-    float v = 0.f;
-    if (c < C) {
-#pragma unroll 8
-        for (int i = s; i < parts; i += 32) v += part[((int64_t)i * 2 + which) * C + c];
+    constexpr int S = 1024 / FOLD;
+    __shared__ float box[FOLD][S + 1];
+    const int j = threadIdx.x % FOLD, s = threadIdx.x / FOLD;
+    const int c = blockIdx.x * FOLD + j, which = blockIdx.y;
+    const float* at = part + (int64_t)which * C + (c < C ? c : 0);
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int i = s + u * S;
+        v[u] = at[(int64_t)(i < parts ? i : 0) * 2 * C];
+        v[u] = i < parts ? v[u] : 0.f;
     }
-    box[s][j] = v;
+    box[j][s] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
     __syncthreads();
-    v = lanes_sum<32>(box[j][s]);                                // thread (s, j): column s, slice j
-    if (j == 0 && blockIdx.x * 32 + s < C) give(which ? dbeta : dgamma, blockIdx.x * 32 + s, v, add & (1 << which));
+    const int wave = threadIdx.x >> 6;                           // a wave a column
+    const float sum = lanes_sum<64>(box[wave][threadIdx.x & 63]);
+    const int col = blockIdx.x * FOLD + wave;
+    if ((threadIdx.x & 63) == 0 && col < C) give(which ? dbeta : dgamma, col, sum, add & (1 << which));
 }
 
 // ---- rows that no workgroup holds (or fewer channels than a chunk): a workgroup walks the row, element by element -------
@@ -519,7 +544,7 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         const int TH = h.L > 512 ? h.L : 512, R = TH / h.L, W = TH / 64;
         const int64_t need = (rows + R - 1) / R;
         const dim3 g((unsigned)(sums ? parts : (need < 2048 ? need : 2048)));
-        const size_t lds = sums && R > 1 ? sizeof(float) * ((R < W ? R : W) * (size_t)C) : 0, box = sizeof(float) * 2 * W;
+        const size_t lds = sums && R > 1 ? sizeof(float) * ((R < W ? R : W) * (size_t)(C % V ? C + (C >> 3) + 1 : C)) : 0, box = sizeof(float) * 2 * W;
         float* pp = parts > 1 ? part : nullptr;
         // x, dy and dx against the last-level cache of 256 MB; read past the caches / through them, us: 30000 x 1024 fp32 (369 MB)
         // 63 / 73, 100000 x 256 fp32 (307 MB) 55 / 58, 16384 x 4096 bf16 (403 MB) 75 / 77; 6144 x 768 bf16 (28 MB) 11.8 / 11.4.
@@ -546,7 +571,7 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         if (sums)
             hipLaunchKernelGGL((ln_columns_kernel<T>), dim3(cdiv(C, 256), parts), dim3(256), 0, st, dy, lddy, x, ldx, mean, rstd, part, rows, C);
     }
-    if (sums) hipLaunchKernelGGL(ln_fold_kernel, dim3(cdiv(C, 32), 2), dim3(1024), 0, st, part, parts, dgamma, dbeta, add, C);
+    if (sums) hipLaunchKernelGGL(ln_fold_kernel, dim3(cdiv(C, FOLD), 2), dim3(1024), 0, st, part, parts, dgamma, dbeta, add, C);
     ADVMIX_CHECK_LAUNCH();
     return ADVMIX_OK;
 }

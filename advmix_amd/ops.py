@@ -1241,34 +1241,37 @@ class LayerNorm:
 
     @staticmethod
     def launch(st, x, gamma, beta, eps, stats):
-        """(y, the fp32 [2, rows] means and rstds or None); x: as LAYOUT leaves it, the arguments checked."""
+        """(y, the fp32 [2, rows] means and rstds or None, (rows, C, distance of x's rows, type)); x: as LAYOUT leaves it, the
+        arguments checked."""
         rows, C = LayerNorm._sizes(x)
         y = LayerNorm._like(x)
         s = torch.empty((2, rows), device=x.device, dtype=torch.float32) if stats else None
+        size = (rows, C, _row_stride(x), _LN_TYPES[x.dtype])
         if rows:
             at = None if s is None else s.data_ptr()
-            rc = lib.advmix_layer_norm_fwd(x.data_ptr(), _row_stride(x), None if gamma is None else gamma.data_ptr(),
+            rc = lib.advmix_layer_norm_fwd(x.data_ptr(), size[2], None if gamma is None else gamma.data_ptr(),
                                            None if beta is None else beta.data_ptr(), y.data_ptr(), at, at and at + 4 * rows, rows,
-                                           C, _LN_TYPES[x.dtype], eps, st)
+                                           C, size[3], eps, st)
             if rc:
                 failed('advmix_layer_norm_fwd', rc)
-        return y, s
+        return y, s, size
 
     @staticmethod
     def fwd(st, lane, t, meta, needs):
         x, gamma, beta = t
         x = LayerNorm.LAYOUT(x)
         LayerNorm.check(x, gamma, beta, meta)
-        y, s = LayerNorm.launch(st, x, gamma, beta, meta, any(needs))
-        return (y,), (() if s is None else (x, gamma, beta, s)), None
+        y, s, size = LayerNorm.launch(st, x, gamma, beta, meta, any(needs))
+        return (y,), (() if s is None else (x, gamma, beta, s)), size
 
     @staticmethod
-    def bwd(st, lane, saved, extra, meta, grads, needs, solo=False):
+    def bwd(st, lane, saved, size, meta, grads, needs, solo=False):
         """``solo``: the launch is on the caller's stream and no other member runs beside it - a parameter's first gradient is
         written instead of added to zeros, and temporaries need not outlive a join."""
         if torch.is_grad_enabled():
             raise RuntimeError('advmix_amd: layer_norm has no second derivative (backward with create_graph=True)')
         x, gamma, beta, s = saved
+        rows, C, ldx, kind = size
         dy = grads[0]
         lddy = _row_stride(dy)
         if lddy is None:
@@ -1276,23 +1279,20 @@ class LayerNorm:
             lddy = _row_stride(dy)
             if not solo:
                 keep(dy)
-        rows, C = LayerNorm._sizes(x)
-        solo = solo and rows > 0
         dx = LayerNorm._like(x) if needs[0] else None
-        dg, add_g = LayerNorm._grad(gamma, st, solo) if needs[1] else (None, 0)
-        db, add_b = LayerNorm._grad(beta, st, solo) if needs[2] else (None, 0)
+        dg, add_g = LayerNorm._grad(gamma, st, solo and rows) if needs[1] else (None, 0)
+        db, add_b = LayerNorm._grad(beta, st, solo and rows) if needs[2] else (None, 0)
         if rows:
-            kind, part = _LN_TYPES[x.dtype], None
+            part = None
             if dg is not None or db is not None:           # (this call's own: two captured graphs must not share it)
-                part = torch.empty(lib.advmix_layer_norm_parts(rows, C, kind) * 2 * C, device=x.device, dtype=torch.float32)
+                part = s.new_empty(lib.advmix_layer_norm_parts(rows, C, kind) * 2 * C)
                 if not solo:
                     keep(part)
             at = s.data_ptr()
-            rc = lib.advmix_layer_norm_bwd(dy.data_ptr(), lddy, x.data_ptr(), _row_stride(x),
-                                           None if gamma is None else gamma.data_ptr(), at, at + 4 * rows,
-                                           None if dx is None else dx.data_ptr(), None if dg is None else dg.data_ptr(),
-                                           None if db is None else db.data_ptr(), None if part is None else part.data_ptr(),
-                                           add_g + 2 * add_b, rows, C, kind, st)
+            rc = lib.advmix_layer_norm_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, None if gamma is None else gamma.data_ptr(),
+                                           at, at + 4 * rows, None if dx is None else dx.data_ptr(),
+                                           None if dg is None else dg.data_ptr(), None if db is None else db.data_ptr(),
+                                           None if part is None else part.data_ptr(), add_g + 2 * add_b, rows, C, kind, st)
             if rc:
                 failed('advmix_layer_norm_bwd', rc)
         return dx, None, None
@@ -1300,10 +1300,12 @@ class LayerNorm:
     @staticmethod
     def _grad(p, st, write=False):
         """(p.grad, 1 if the kernel has to add to it, 0 if it has to write it)."""
-        if write and p.grad is None and getattr(p, '_flat_grad_view', None) is None:
-            p.grad = torch.empty_like(p)
-            return p.grad, 0
-        g = _grad_buf(p, st)
+        g = p.grad
+        if g is None:
+            if write and getattr(p, '_flat_grad_view', None) is None:
+                g = p.grad = torch.empty_like(p)
+                return g, 0
+            g = _grad_buf(p, st)
         if g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape or g.device != p.device:
             raise RuntimeError('layer_norm: a parameter\'s .grad must be a contiguous fp32 tensor of its shape')
         return g, 1
@@ -1326,21 +1328,20 @@ class LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, gamma, beta, eps, params, wants):
         if params is not None:
             gamma, beta = params
-        y, s = LayerNorm.launch(_raw_stream(x.device.index), x, gamma, beta, eps, True)
+        y, s, size = LayerNorm.launch(_raw_stream(x.device.index), x, gamma, beta, eps, True)
         ctx.save_for_backward(x)
         ctx.set_materialize_grads(False)
-        ctx.rest = (gamma, beta, s, None if gamma is None else gamma._version)
-        ctx.wants = wants
+        ctx.rest = (gamma, beta, s, size, wants, None if gamma is None else gamma._version)
         return y
 
     @staticmethod
     def backward(ctx, dy):
         if dy is None:
             return None, None, None, None, None, None
-        gamma, beta, s, version = ctx.rest
+        gamma, beta, s, size, wants, version = ctx.rest
         if gamma is not None and gamma._version != version:
             raise RuntimeError('layer_norm: gamma was modified in place between the forward and the backward pass')
-        dx = LayerNorm.bwd(_raw_stream(dy.device.index), 0, ctx.saved_tensors + (gamma, beta, s), None, None, (dy,), ctx.wants, solo=True)[0]
+        dx = LayerNorm.bwd(_raw_stream(dy.device.index), 0, ctx.saved_tensors + (gamma, beta, s), size, None, (dy,), wants, True)[0]
         return dx, None, None, None, None, None
 
 
