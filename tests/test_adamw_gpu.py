@@ -407,6 +407,47 @@ def test_layer_norms_trained_with_adamw(bits):
             assert float((p.detach().double().cpu() - q.detach()).abs().max()) <= 1e-4 * (it + 1)
 
 
+@pytest.mark.parametrize('bits,clip', [(32, None), (8, 1.0)])
+def test_advmix_step_as_graphs_and_eager(bits, clip):
+    """The AdvMix step with FlatAdamW for both networks, deterministic mode: three batches through AdvMixGraphRunner (warm-up,
+    snapshot, restore, replays) leave the bits that the eager step leaves."""
+    import types
+    from advmix_amd import ops
+    from advmix_amd.core.function import advmix_step
+    from advmix_amd.graph import AdvMixGraphRunner
+    from advmix_amd.utils.utils import adamw_groups
+    from oracle.synth import synth_batch
+    from test_models_gpu import _tiny_setup
+    args = types.SimpleNamespace(alpha=0.1, adv_loss_weight=1.0)
+    data = []
+    for it in range(3):
+        v, t, w = synth_batch('hrnet_tiny.it%d' % (it % 2), 2, 5, 64, 64)
+        data.append(([x.cuda().contiguous() for x in v], t.cuda(), w.cuda()))
+
+    def nets():
+        _, D, G, T, crit, _, _, _ = _tiny_setup(lr=1e-3)
+        return (D, G, T, crit) + tuple(AdamW(adamw_groups(m, 0.05), lr=1e-3, state_bits=bits, max_norm=clip, seed=k) for k, m in enumerate((D, G)))
+    try:
+        ops.set_deterministic(True)
+        D, G, T, crit, oD, oG = nets()
+        runner = AdvMixGraphRunner(args, D, G, T, crit, oD, oG, *data[0], warmup=2)
+        losses = []
+        for batch in data:
+            runner.load_batch(*batch)
+            loss, _ = runner.step()
+            losses.append(float(loss))
+        torch.cuda.synchronize()
+        D2, G2, T2, crit2, oD2, oG2 = nets()
+        for batch, loss in zip(data, losses):
+            l2, _ = advmix_step(args, D2, G2, T2, crit2, oD2, oG2, *batch)
+            assert float(l2) == loss
+    finally:
+        ops.set_deterministic(False)
+    for a, b in ((oD, oD2), (oG, oG2)):
+        assert int(a.flat_state()[3]) == 3
+        assert all(torch.equal(x, y) for x, y in zip(a.flat_state(), b.flat_state()))
+
+
 def test_get_optimizer_trains_a_pose_net():
     """TRAIN.OPTIMIZER adamw through get_optimizer: groups, and one plain_step of a small pose net moves every tensor."""
     import types

@@ -269,6 +269,49 @@ def test_between_other_ops():
         assert float((a.detach().double().cpu() - b.detach()).abs().max()) <= 1e-4 * float(b.detach().abs().max())
 
 
+def test_twice_through_one_graph_and_without_the_leaf():
+    """retain_graph: the second pass adds; autograd.grad for x alone leaves x.grad alone; gamma changed in between is refused."""
+    x, dy, gamma, beta = inputs((50, 130), torch.float32)
+    x.requires_grad_()
+    y = ops().layer_norm(x, gamma, beta)
+    y.backward(dy, retain_graph=True)
+    first = [t.grad.clone() for t in (x, gamma, beta)]
+    y.backward(dy, retain_graph=True)
+    assert all(torch.equal(t.grad, 2 * f) for t, f in zip((x, gamma, beta), first))
+    x.grad = None
+    (dx,) = torch.autograd.grad(y, x, dy, retain_graph=True)
+    assert x.grad is None and torch.equal(dx, first[0])
+    with torch.no_grad():
+        gamma.add_(1.0)
+    with pytest.raises(RuntimeError):
+        y.backward(dy)
+    y = ops().layer_norm(x, gamma, beta)
+    with torch.no_grad():
+        x.add_(1.0)
+    with pytest.raises(RuntimeError):
+        y.backward(dy)
+
+
+def test_inside_a_chain():
+    """A chain of two layer norms on one lane, their shared input's gradient summed in the chain."""
+    o = ops()
+    x, dy, g1, b1 = inputs((2, 24, 6, 5), torch.float32)
+    g2, b2 = (torch.nn.Parameter((1 + 0.3 * rand(24, seed=s)).to(dev())) for s in (8, 9))
+    x.requires_grad_()
+    subs = ((o.LayerNorm, (('s', 0), ('i', 1), ('i', 2)), 1e-5, 1), (o.LayerNorm, (('s', 1), ('i', 3), ('i', 4)), 1e-5, 2))
+    (y,) = o.run_group([(o.Chain, (x, g1, b1, g2, b2), (subs, (0,), (2,)))])[0]
+    y.backward(dy)
+    xr, pr = x.detach().double().cpu().requires_grad_(), [p.detach().double().cpu().requires_grad_() for p in (g1, b1, g2, b2)]
+
+    def norm(t, g, b):
+        d = t - t.mean(1, keepdim=True)
+        return d / (d.square().mean(1, keepdim=True) + 1e-5).sqrt() * g.view(-1, 1, 1) + b.view(-1, 1, 1)
+    yr = norm(norm(xr, *pr[:2]), *pr[2:])
+    yr.backward(dy.double().cpu())
+    for a, b in ((y, yr), (x.grad, xr.grad), *((p.grad, q.grad) for p, q in zip((g1, b1, g2, b2), pr))):
+        assert float((a.detach().double().cpu() - b.detach()).abs().max()) <= 1e-5 * (1 + float(b.detach().abs().max()))
+
+
 def test_captured_and_replayed():
     """Two graphs, replayed in turn with eager work of the same sizes between: each replay gives the eager bits."""
     o = ops()
