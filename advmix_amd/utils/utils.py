@@ -314,17 +314,18 @@ class FlatAdamW(FlatAdam):
         super()._ensure_flat()
         fp, _, m, v = self._flat
         dev = fp.device
-        group = {id(p): k for k, g in enumerate(self.param_groups) for p in g['params']}
-        rows, self._chunks, self._blocks, block = [], [], [], 0
-        for p, off in zip(self._params(), self._offsets):
-            n = _ceil4(p.numel())
-            first, first_block = len(rows), block
-            for k in range(0, n, self.CHUNK):
-                rows.append((off + k, min(self.CHUNK, n - k), group[id(p)], block + k // self.BLOCK))
-            block += -(-n // self.BLOCK)
-            self._chunks.append((first, len(rows)))
-            self._blocks.append((first_block, block))
-        self._table = torch.tensor(rows, dtype=torch.int64).to(dev)
+        # the chunk table, tensor by tensor: {first element, elements, group, first block of scales}
+        of_group = torch.tensor([k for k, g in enumerate(self.param_groups) for _ in g['params']])
+        first, n = torch.tensor(self._offsets), torch.tensor([_ceil4(p.numel()) for p in self._params()])
+        chunks, blocks = -(-n // self.CHUNK), -(-n // self.BLOCK)
+        ends, block_ends = chunks.cumsum(0), blocks.cumsum(0)
+        self._chunks = list(zip((ends - chunks).tolist(), ends.tolist()))
+        self._blocks = list(zip((block_ends - blocks).tolist(), block_ends.tolist()))
+        of = torch.repeat_interleave(torch.arange(len(n)), chunks)                     # a chunk's tensor
+        at = (torch.arange(len(of)) - (ends - chunks)[of]) * self.CHUNK                # where in it the chunk begins
+        self._table = torch.stack([first[of] + at, torch.clamp(n[of] - at, max=self.CHUNK), of_group[of],
+                                   (block_ends - blocks)[of] + at // self.BLOCK], 1).contiguous().to(dev)
+        block = self._blocks[-1][1]
         self._hyper = torch.tensor(self._hyper_host, dtype=torch.float64).to(dev)
         self._coef = torch.zeros(8 * len(self.param_groups) + 8, device=dev, dtype=torch.float32)
         self._parts = torch.empty(self.PARTS, device=dev, dtype=torch.float64) if self._clips else None
@@ -335,7 +336,7 @@ class FlatAdamW(FlatAdam):
         self._index, self._ps, self._raw_host = dev.index, self._params(), self._hyper_raw()
         fp, fg, m, v = self._flat                             # (these buffers live as long as the optimizer)
         P = lambda t: None if t is None else t.data_ptr()          # noqa: E731
-        rest = (P(self._table), len(rows), P(self._hyper), len(self.param_groups), P(self._step), P(self._parts),
+        rest = (P(self._table), len(self._table), P(self._hyper), len(self.param_groups), P(self._step), P(self._parts),
                 self.PARTS if self._clips else 0, P(self.grad_norm))
         if self.state_bits == 8:
             self._step_args = ('advmix_adamw8', P(fp), P(fg), P(m), P(v), *map(P, self._scales), *rest, self.seed, P(self._coef))
