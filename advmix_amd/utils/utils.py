@@ -253,7 +253,7 @@ class FlatAdamW(FlatAdam):
     ``state_dict`` holds exp_avg / exp_avg_sq as torch.optim does, or with 8 bits exp_avg_codes / exp_avg_scale and
     exp_avg_root_codes / exp_avg_root_scale as they are; either kind of optimizer loads either kind of state."""
 
-    CHUNK, BLOCK, HYPER, PARTS = 1024, 256, 8, 1024
+    CHUNK, BLOCK, HYPER = 1024, 256, 8
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=None, seed=0):
         if state_bits not in (8, 32):
@@ -328,7 +328,8 @@ class FlatAdamW(FlatAdam):
         block = self._blocks[-1][1]
         self._hyper = torch.tensor(self._hyper_host, dtype=torch.float64).to(dev)
         self._coef = torch.zeros(8 * len(self.param_groups) + 8, device=dev, dtype=torch.float32)
-        self._parts = torch.empty(self.PARTS, device=dev, dtype=torch.float64) if self._clips else None
+        nparts = max(1, min(1024, fp.numel() // 4096)) if self._clips else 0           # (of the norm: a workgroup each)
+        self._parts = torch.empty(nparts, device=dev, dtype=torch.float64) if self._clips else None
         self.grad_norm = torch.zeros((), device=dev, dtype=torch.float32) if self._clips else None
         if self.state_bits == 8:
             self._flat = self._flat[:2] + tuple(torch.zeros(fp.numel(), device=dev, dtype=torch.uint8) for _ in range(2))
@@ -337,20 +338,20 @@ class FlatAdamW(FlatAdam):
         fp, fg, m, v = self._flat                             # (these buffers live as long as the optimizer)
         P = lambda t: None if t is None else t.data_ptr()          # noqa: E731
         rest = (P(self._table), len(self._table), P(self._hyper), len(self.param_groups), P(self._step), P(self._parts),
-                self.PARTS if self._clips else 0, P(self.grad_norm))
+                nparts, P(self.grad_norm))
         if self.state_bits == 8:
             self._step_args = ('advmix_adamw8', P(fp), P(fg), P(m), P(v), *map(P, self._scales), *rest, self.seed, P(self._coef))
         else:
             self._step_args = ('advmix_adamw', P(fp), P(fg), P(m), P(v), *rest, P(self._coef))
-        self._norm_args = (P(fg), fg.numel(), P(self._parts), self.PARTS)
+        self._norm_args = (P(fg), fg.numel(), P(self._parts), nparts)
 
     def flat_state(self):
         """[parameters, m, v, step]; with 8 bits [parameters, m codes, r codes, step, m exponent bytes, r exponent bytes]."""
         return super().flat_state() + (list(self._scales) if self.state_bits == 8 else [])
 
     def _hyper_raw(self):
-        return [self.max_norm] + [x for g in self.param_groups for x in (
-            float(g['lr']), g['betas'], g['eps'], g['weight_decay'], g.get('amsgrad'), g.get('maximize'))]
+        return [self.max_norm if self.max_norm is None else float(self.max_norm)] + [x for g in self.param_groups for x in (
+            float(g['lr']), *map(float, g['betas']), float(g['eps']), float(g['weight_decay']), g.get('amsgrad'), g.get('maximize'))]
 
     def sync_hyper(self):
         self._ensure_flat()
@@ -374,17 +375,21 @@ class FlatAdamW(FlatAdam):
 
     @torch.no_grad()
     def step(self, closure=None, sync_hyper=True):
-        if closure is not None:
-            raise ValueError('FlatAdamW: step() takes no closure')
         self._ensure_flat()
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
         if sync_hyper and not torch.cuda.is_current_stream_capturing():
             self.sync_hyper()
         self._attach_grads(strict=True)
         index = self._index
         if index != torch.cuda.current_device():
             with torch.cuda.device(index):
-                return self._launch(index)
-        self._launch(index)
+                self._launch(index)
+        else:
+            self._launch(index)
+        return loss
 
     def _launch(self, index):
         st = torch.cuda.current_stream(index).cuda_stream
@@ -430,8 +435,11 @@ class FlatAdamW(FlatAdam):
                 if full in st:
                     if st[full].shape != p.shape:
                         raise ValueError('FlatAdamW: %s of parameter %d has another shape' % (full, i))
-                elif codes not in st or scale not in st or st[codes].shape != p.shape or st[scale].numel() != hi - lo:
-                    raise ValueError('FlatAdamW: the state of parameter %d lacks %s, or its codes have another shape' % (i, full))
+                elif codes not in st or scale not in st or st[codes].shape != p.shape or st[scale].numel() != hi - lo \
+                        or st[codes].dtype not in (torch.float8_e4m3fn, torch.uint8) \
+                        or st[scale].dtype not in (torch.float8_e8m0fnu, torch.uint8):
+                    raise ValueError('FlatAdamW: the state of parameter %d lacks %s, or its codes have another shape or type' % (i, full))
+            float(st['step'])
             todo.append((i, p, st))
         before = [dict(g) for g in self.param_groups]
         for g, new in zip(self.param_groups, sd['param_groups']):

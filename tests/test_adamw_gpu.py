@@ -360,10 +360,13 @@ def test_refusals_on_the_device():
     with pytest.raises(ValueError):
         o.step()
     o.param_groups[0]['lr'] = 1e-3
-    with pytest.raises(ValueError):
-        o.step(lambda: 0.0)
     sd = o.state_dict()
-    for spoil in (lambda s: s['state'][0].pop('exp_avg'), lambda s: s['state'][0].update(exp_avg=torch.zeros(9)),
+    codes = dict(step=1.0, exp_avg_codes=torch.zeros(8, dtype=torch.uint8), exp_avg_scale=torch.zeros(1, dtype=torch.uint8),
+                 exp_avg_root_codes=torch.zeros(8, dtype=torch.uint8), exp_avg_root_scale=torch.zeros(1, dtype=torch.uint8))
+    for spoil in (lambda s: s['state'].update({0: dict(codes, exp_avg_codes=torch.zeros(8))}),
+                  lambda s: s['state'].update({0: dict(codes, exp_avg_scale=torch.zeros(2, dtype=torch.uint8))}),
+                  lambda s: s['state'].update({0: dict(codes, exp_avg_root_codes=torch.zeros(9, dtype=torch.uint8))}),
+                  lambda s: s['state'][0].pop('exp_avg'), lambda s: s['state'][0].update(exp_avg=torch.zeros(9)),
                   lambda s: s.update(param_groups=s['param_groups'] * 2), lambda s: s['param_groups'][0].update(eps=0.0)):
         s = copy.deepcopy(sd)
         spoil(s)
@@ -371,6 +374,31 @@ def test_refusals_on_the_device():
             o.load_state_dict(s)
     assert o.param_groups[0]['eps'] == 1e-8
     o.step()
+
+
+def test_closure_and_scheduler():
+    """step(closure) computes the gradients and hands the loss back; a torch scheduler drives the learning rate."""
+    w = torch.nn.Parameter(torch.ones(4, 8, device=dev()))
+    o = AdamW([w], lr=0.1, weight_decay=0.0, eps=1e-8)
+    sched = torch.optim.lr_scheduler.MultiStepLR(o, [1], 0.1)
+    x = rand_like(w)
+
+    def closure():
+        o.zero_grad()
+        loss = (w * x).sum()
+        loss.backward()
+        return loss
+    for lr in (0.1, 0.01):
+        before = w.detach().clone()
+        loss = o.step(closure)
+        assert abs(float(loss) - float((before.double() * x.double()).sum())) <= 1e-4
+        # a constant gradient: m / sqrt(v) is its sign after bias correction
+        assert float((w.detach() - (before - lr * x.sign())).abs().max()) <= 1e-5
+        sched.step()
+
+
+def rand_like(t):
+    return torch.randn(*t.shape, generator=torch.Generator().manual_seed(5)).to(t.device)
 
 
 @pytest.mark.parametrize('bits', [32, 8])

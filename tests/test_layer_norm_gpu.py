@@ -350,6 +350,32 @@ def test_captured_and_replayed():
             assert torch.equal(a, b), k
 
 
+@pytest.mark.parametrize('leaf', [True, False])
+def test_captured_while_an_eager_graph_of_the_parameters_is_alive(leaf):
+    """gamma and beta are no inputs of the node: an eager graph of theirs (on the default stream, kept) does not reach a capture."""
+    o = ops()
+    x, dy, gamma, beta = inputs((64, 96), torch.float32)
+    kept = o.layer_norm(x.clone().requires_grad_(), gamma, beta)
+    kept.backward(dy, retain_graph=True)
+    want = [gamma.grad.clone(), beta.grad.clone()]
+    other = x.clone().requires_grad_(leaf)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        o.layer_norm(x.clone().requires_grad_(leaf), gamma, beta).backward(dy)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o.layer_norm(other, gamma, beta).backward(dy)       # adds to the gradients that are there
+    for _ in range(3):
+        gamma.grad.zero_()
+        beta.grad.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(gamma.grad, want[0]) and torch.equal(beta.grad, want[1])
+    assert kept.grad_fn is not None
+
+
 def test_on_another_stream():
     x, dy, gamma, beta = inputs((900, 300), torch.float32)
     x.requires_grad_()
