@@ -8,8 +8,10 @@
 // chosen so that the block's largest finite magnitude lies in [128, 256).  A power of two keeps values that do not change on
 // the grid when the scale moves.  Rounding: up if the fraction between two codes plus u is 1 or more, u in [0, 1) from a hash of
 // the element's place, the step and a seed.  Nearest rounding would freeze r - a step moves it by 0.05 %, half a code is 3 - 6 % -
-// while a value that the step hardly moves picks up hardly any noise this way (probability |change| / code distance).  r > 0 is
-// held as no less than the smallest code, so that no denominator collapses.
+// while a value that the step hardly moves picks up hardly any noise this way (probability |change| / code distance).  600 steps
+// of the formulas over 4096 elements, b2 = 0.999: the average of r^2 stays within 4 % of v's (one element's spreads by up to 36 %)
+// and the weights' path within 14 %; with nearest rounding r^2 is 36 - 54 % low and the path 33 % off.  r > 0 is held as no less
+// than the smallest code, so that no denominator collapses.
 // The moments' arithmetic is rounded operation by operation (no fused multiply-add), so that codes are reproducible from the formula.
 #include "common.h"
 
@@ -71,10 +73,12 @@ __global__ __launch_bounds__(256) void tick_kernel(const double* __restrict__ hy
                                                    uint32_t seed, float* __restrict__ coef) {
     __shared__ double red[4];
     const int64_t t = *step + 1;
-    double s = 0.0;
-    for (int i = threadIdx.x; i < nparts; i += 256) s += part[i];
-    s = wave_sum_d(s);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if (part) {
+        double s = 0.0;
+        for (int i = threadIdx.x; i < nparts; i += 256) s += part[i];
+        s = wave_sum_d(s);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    }
     __syncthreads();                                             // (also: everyone has read *step)
     float clip = 1.f;
     if (part) {

@@ -234,7 +234,7 @@ __device__ __forceinline__ void give(float* to, int64_t c, float v, int add) {
 
 // part[workgroup][0][c] = sum of dy * xh, [1][c] = sum of dy over the workgroup's rows; a launch of one workgroup gives its sums
 // to dgamma and dbeta itself (part NULL).
-// PAST: x and dy are read past the caches (both are dead after this kernel).
+// PAST: x is read past the caches (dy is what another kernel has just left there).
 template <typename T, int L, int NV, bool TAIL, bool PAST>
 __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
                                                                  int64_t ldx, const float* __restrict__ gamma,
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
         for (int k = 0; k < NV; ++k) {
             const int at = Place<V, L, TAIL>(k, l, C).at;
             nw[k] = PAST ? load_past(xr + at) : load(xr + at);
-            ng[k] = PAST ? load_past(gr + at) : load(gr + at);
+            ng[k] = load(gr + at);
         }
     };
     if (ROOM) fetch(r);
@@ -546,9 +546,9 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         const dim3 g((unsigned)(sums ? parts : (need < 2048 ? need : 2048)));
         const size_t lds = sums && R > 1 ? sizeof(float) * ((R < W ? R : W) * (size_t)(C % V ? C + (C >> 3) + 1 : C)) : 0, box = sizeof(float) * 2 * W;
         float* pp = parts > 1 ? part : nullptr;
-        // x, dy and dx against the last-level cache of 256 MB; read past the caches / through them, us: 30000 x 1024 fp32 (369 MB)
-        // 63 / 73, 100000 x 256 fp32 (307 MB) 55 / 58, 16384 x 4096 bf16 (403 MB) 75 / 77; 6144 x 768 bf16 (28 MB) 11.8 / 11.4.
-        // (Odd widths keep to the caches, where neighbouring rows share lines.)
+        // x, dy and dx against the last-level cache of 256 MB.  x read past the caches / through them, us: 30000 x 1024 fp32 (369 MB)
+        // 61 / 71, 100000 x 256 fp32 (307 MB) 52 / 56, 16384 x 4096 bf16 (403 MB) 78 / 79; 6144 x 768 bf16 (28 MB) 11.8 / 11.4.  With
+        // dy past them too the pass behind a forward pass loses 6 - 12 %.  (Odd widths keep to the caches: neighbouring rows share lines.)
         const bool past = rows * C * (int64_t)sizeof(T) * 3 > (256ll << 20);
 #define BWD(L_, NV_)                                                                                                             \
     if (h.L == L_ && h.NV == NV_) {                                                                                              \

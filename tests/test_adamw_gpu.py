@@ -391,7 +391,7 @@ def test_closure_and_scheduler():
     for lr in (0.1, 0.01):
         before = w.detach().clone()
         loss = o.step(closure)
-        assert abs(float(loss) - float((before.double() * x.double()).sum())) <= 1e-4
+        assert abs(float(loss.detach()) - float((before.double() * x.double()).sum())) <= 1e-4
         # a constant gradient: m / sqrt(v) is its sign after bias correction
         assert float((w.detach() - (before - lr * x.sign())).abs().max()) <= 1e-5
         sched.step()
