@@ -506,7 +506,7 @@ int advmix_fill(float* p, float value, int64_t n, void* stream);
  * hyper (device): double [1 + groups][8]; row 0 = {max_norm}, row 1 + k = {lr, b1, b2, eps, weight decay} of group k.
  * step (device int64) is incremented by the launch (graph-replay safe).  part: NULL (no clipping, nparts 0) or what
  *   advmix_grad_sumsq left; then the gradient's norm before clipping goes to norm_out.  coef: 4 * (8 * groups + 8) bytes of
- *   scratch that belongs to this optimizer alone. */
+ *   scratch that belongs to this optimizer alone, zero before the first step. */
 int advmix_adamw(float* p, const float* g, float* m, float* v, const int64_t* table, int chunks, const double* hyper, int groups,
                  int64_t* step, const double* part, int nparts, float* norm_out, float* coef, void* stream);
 /* The same step on 8-bit moments: m and r = sqrt(v) as e4m3 codes, blocks of 256 elements within a tensor, each with an

@@ -139,6 +139,49 @@ def test_8_bit_step_matches_the_formula(seed, clip):
             assert (np.abs(flat(p) - want) <= tol).all(), (t, i, float((np.abs(flat(p) - want) / tol).max()))
 
 
+@pytest.mark.parametrize('sizes', [(100001, 7), (130000, 77), (300001, 1025), (17000001, 3000)], ids=str)
+@pytest.mark.parametrize('bits', [32, 8])
+def test_larger_steps(bits, sizes):
+    """Small steps (no launch before theirs), larger ones, and ones past the caches: two clipped steps, all elements."""
+    g = torch.Generator(device=dev()).manual_seed(2)
+    ps = [torch.nn.Parameter(torch.randn(n, device=dev(), generator=g)) for n in sizes]
+    o = AdamW([dict(params=[ps[0]], weight_decay=0.1), dict(params=[ps[1]], lr=3e-3, weight_decay=0.0)], betas=(0.9, 0.99),
+              state_bits=bits, max_norm=1.0, seed=5)
+    for t in (1, 2):
+        for p in ps:
+            p.grad.copy_(torch.randn(p.shape, device=dev(), generator=g) * 1e-2)
+        norm = float(sum((p.grad.double() ** 2).sum() for p in ps).sqrt())
+        c = float(np.float32(min(1.0, 1.0 / (norm + 1e-6))))
+        before = [(p.detach().double().cpu().numpy(), p.grad.cpu().numpy()) for p in ps]
+        states = [t_.clone() for t_ in o.flat_state()]
+        o.step()
+        assert abs(float(o.grad_norm) - norm) <= 4 * U * norm and int(o.flat_state()[3]) == t
+        for k, p in enumerate(ps):
+            n, off, (lo, hi) = p.numel(), p._flat_off, o._blocks[k]
+            p0, gr = before[k]
+            gr = gr * np.float32(c)
+            cut = lambda x: x[off:off + n].cpu()          # noqa: E731
+            if bits == 32:
+                m0, v0 = (cut(x).double().numpy() for x in states[1:3])
+            else:
+                val = lambda x, e: cut(x).view(torch.float8_e4m3fn).double().numpy() * np.repeat(2.0 ** (e[lo:hi].cpu().double().numpy() - 127), 256)[:n]          # noqa: E731
+                m0, v0 = val(states[1], states[4]), val(states[2], states[5]) ** 2
+            m1, v1, m, v = plain.moments(m0, v0, gr.astype(np.float64), 0.9, 0.99)
+            now = o.flat_state()
+            if bits == 32:                                  # (the same operations, each rounded)
+                assert np.array_equal(cut(now[1]).numpy(), m1) and np.array_equal(cut(now[2]).numpy(), v1)
+            else:
+                um, ur = plain.dither(np.arange(n) + off, t, 5)
+                for x, u, least, codes, scale in ((m1, um, 0.0, now[1], now[4]), (np.sqrt(v1), ur, 2.0 ** -9, now[2], now[5])):
+                    want, E = plain.hold(x, u, least)
+                    assert np.array_equal(scale[lo:hi].cpu().numpy(), E)
+                    assert np.array_equal(cut(codes).view(torch.float8_e4m3fn).double().numpy(), want)
+            lr, wd = (1e-3, 0.1) if k == 0 else (3e-3, 0.0)
+            want = plain.weights(p0, m, v, t, lr, 0.9, 0.99, 1e-8, wd)
+            tol = 2 * U * np.abs(p0) + 20 * U * np.abs(want - p0) + 200 * U * lr * (1 + np.abs(m0) / np.maximum(np.sqrt(v), 1e-30))
+            assert (np.abs(p.detach().double().cpu().numpy() - want) <= tol).all()
+
+
 def test_8_bit_moments_follow_the_32_bit_ones():
     """600 steps of random gradients that shrink on the way.  The formulas in 64 bits give: the average of r^2 over 4096 elements is
     1.036 of v's, one element's ratio spreads by 0.36 (so the average by 0.006; five times that is allowed), and the weights are
