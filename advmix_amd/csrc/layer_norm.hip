@@ -233,7 +233,7 @@ __device__ __forceinline__ void give(float* to, int64_t c, float v, int add) {
 }
 
 // part[workgroup][0][c] = sum of dy * xh, [1][c] = sum of dy over the workgroup's rows; a launch of one workgroup gives its sums
-// to dgamma and dbeta itself (part NULL).
+// to dgamma and dbeta itself (part NULL; not one of long rows, whose lanes would write them one element at a time).
 // PAST: x is read past the caches (dy is what another kernel has just left there).
 template <typename T, int L, int NV, bool TAIL, bool PAST>
 __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
@@ -319,20 +319,23 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
         }
     }
     if (!dgamma && !dbeta) return;
-    if (R == 1) {                                                // one row at a time: a lane has its columns to itself
+    if (R == 1) {                                                // one row at a time: a lane has its columns to itself (part is there)
+        typedef f32x4 Four __attribute__((aligned(4)));
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const Place<V, L, TAIL> at(k, l, C);
+        for (int which = 0; which < 2; ++which) {
+            float* row = part + ((int64_t)blockIdx.x * 2 + which) * C;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if (!(TAIL ? e >= at.from : at.any)) continue;
-                const int c = at.at + e;
-                if (part) {
-                    part[(int64_t)blockIdx.x * 2 * C + c] = dg[k][e];
-                    part[((int64_t)blockIdx.x * 2 + 1) * C + c] = db[k][e];
+            for (int k = 0; k < NV; ++k) {
+                const Place<V, L, TAIL> at(k, l, C);
+                const float(&v)[V] = which ? db[k] : dg[k];
+                if (at.from == 0) {
+#pragma unroll
+                    for (int q = 0; q < V; q += 4)
+                        *reinterpret_cast<Four*>(row + at.at + q) = f32x4{v[q], v[q + 1], v[q + 2], v[q + 3]};
                 } else {
-                    give(dgamma, c, dg[k][e], add & 1);
-                    give(dbeta, c, db[k][e], add & 2);
+#pragma unroll
+                    for (int e = 0; e < V; ++e)
+                        if (e >= at.from) row[at.at + e] = v[e];       // (from = V where the chunk lies behind the row)
                 }
             }
         }
@@ -492,6 +495,7 @@ int parts_of(int64_t rows, int C, int V) {
     if (h.L == 0) return (int)(rows < 256 ? rows : 256);         // column kernel: slices of the rows
     const int R = (h.L > 512 ? h.L : 512) / h.L;
     const int64_t units = (rows + R - 1) / R, most = h.L == 1024 || h.NV * V >= 16 ? 256 : 512;
+    if (R > 1 && units <= 2) return 1;                           // (one workgroup, no folding: 16 x 768 bf16 5.3 us, 6.3 with two)
     const int64_t each = (units + most - 1) / most;
     return (int)((units + each - 1) / each);
 }
@@ -545,7 +549,7 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         const int64_t need = (rows + R - 1) / R;
         const dim3 g((unsigned)(sums ? parts : (need < 2048 ? need : 2048)));
         const size_t lds = sums && R > 1 ? sizeof(float) * ((R < W ? R : W) * (size_t)(C % V ? C + (C >> 3) + 1 : C)) : 0, box = sizeof(float) * 2 * W;
-        float* pp = parts > 1 ? part : nullptr;
+        float* pp = parts > 1 || R == 1 ? part : nullptr;
         // x, dy and dx against the last-level cache of 256 MB.  x read past the caches / through them, us: 30000 x 1024 fp32 (369 MB)
         // 61 / 71, 100000 x 256 fp32 (307 MB) 52 / 56, 16384 x 4096 bf16 (403 MB) 78 / 79; 6144 x 768 bf16 (28 MB) 11.8 / 11.4.  With
         // dy past them too the pass behind a forward pass loses 6 - 12 %.  (Odd widths keep to the caches: neighbouring rows share lines.)
@@ -562,7 +566,7 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         HOLDS(BWD)
         if constexpr (V == 4) { HOLDS_F32(BWD) }
 #undef BWD
-        if (!sums || parts == 1) { ADVMIX_CHECK_LAUNCH(); return ADVMIX_OK; }
+        if (!sums || !pp) { ADVMIX_CHECK_LAUNCH(); return ADVMIX_OK; }
     } else {
         if (dx) {
             if (C < V) hipLaunchKernelGGL((ln_dx_walk_kernel<T, 64>), dim3((unsigned)(rows < 8192 ? rows : 8192)), dim3(64), 0, st, dy, lddy, x, ldx, gamma, mean, rstd, dx, rows, C);
