@@ -140,8 +140,12 @@ template <int V, int L, bool TAIL> struct Place {
         at = TAIL ? (c < C - V ? c : C - V) : (any ? c : 0);
         from = any ? c - at : V;
     }
-    __device__ __forceinline__ float only(float v, int e) const { return (TAIL ? e >= from : any) ? v : 0.f; }
+    // v for an element that is this lane's, 0 for one that another lane sums; a chunk behind the row is left to the caller
+    __device__ __forceinline__ float own(float v, int e) const { return !TAIL || e >= from ? v : 0.f; }
 };
+__device__ __forceinline__ u32x4 zero_unless(bool yes, const u32x4& w) {
+    return yes ? w : u32x4{0u, 0u, 0u, 0u};
+}
 
 // V elements of gamma or beta (``none`` where there is no such tensor); one uniform branch a chunk, so that all loads are in
 // flight together.
@@ -198,19 +202,23 @@ __global__ __launch_bounds__(threads_of(L)) void ln_fwd_kernel(const T* __restri
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const Place<V, L, TAIL> at(k, l, C);
+            float part = 0.f;
 #pragma unroll
-            for (int e = 0; e < V; ++e) s += at.only(Vec<T>::get(w[k], e), e);
+            for (int e = 0; e < V; ++e) part += at.own(Vec<T>::get(w[k], e), e);
+            s += at.any ? part : 0.f;
         }
         const float mu = row_sum<L, TH>(s, box, flip) / n;
         float q = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const Place<V, L, TAIL> at(k, l, C);
+            float part = 0.f;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float d = at.only(Vec<T>::get(w[k], e) - mu, e);
-                q = fmaf(d, d, q);
+                const float d = at.own(Vec<T>::get(w[k], e) - mu, e);
+                part = fmaf(d, d, part);
             }
+            q += at.any ? part : 0.f;
         }
         const float is = 1.f / sqrtf(row_sum<L, TH>(q, box, flip) / n + eps);
 #pragma unroll
@@ -277,12 +285,13 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
     for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < rows; r0 += step, r += step) {
         const bool in = r < rows;
         if (!ROOM) fetch(r);
-        const float mu = nmu, is = nis;
+        // without a row: xh = 0 and dy = 0, whatever the last row holds; behind the row (a chunk of none): dy = 0
+        const float mu = in ? nmu : 0.f, is = in ? nis : 0.f;
         u32x4 w[NV], g[NV];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            w[k] = nw[k];
-            g[k] = ng[k];
+            w[k] = zero_unless(in, nw[k]);
+            g[k] = zero_unless(in && Place<V, L, TAIL>(k, l, C).any, ng[k]);
         }
         if (ROOM && r0 + step < rows) fetch(r + step);
         float a = 0.f, b = 0.f;
@@ -293,16 +302,15 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float xh = (Vec<T>::get(w[k], e) - mu) * is;
-                const float d = in ? at.only(Vec<T>::get(g[k], e), e) : 0.f, h = d * gm[k][e];
-                const float hx = at.only(h * xh, e), dx_ = (in ? at.only(d * xh, e) : 0.f);
+                const float d = at.own(Vec<T>::get(g[k], e), e), h = d * gm[k][e];
                 a += h;
-                b += hx;
-                dg[k][e] += dx_;
+                b = fmaf(h, xh, b);
+                dg[k][e] = fmaf(d, xh, dg[k][e]);                // (of elements that are another lane's, never used)
                 db[k][e] += d;
             }
         }
-        a = row_sum<L, TH>(a, lds, flip) / n;
-        b = row_sum<L, TH>(b, lds, flip) / n;
+        a = row_sum<L, TH>(a, lds, flip) / n * is;
+        b = row_sum<L, TH>(b, lds, flip) / n * is;
         if (dx) {
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -312,7 +320,7 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const float xh = (Vec<T>::get(w[k], e) - mu) * is;
-                    o[e] = is * (Vec<T>::get(g[k], e) * gm[k][e] - a - xh * b);
+                    o[e] = fmaf(Vec<T>::get(g[k], e) * gm[k][e], is, -fmaf(xh, b, a));
                 }
                 if (in && at.any) store(dx + r * C + at.at, Vec<T>::put(o));
             }
