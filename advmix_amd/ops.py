@@ -10,7 +10,7 @@ them.  ``needs_input_grad`` carries the reference's three gradient modes (full /
 after ``set_require_grad(model, False)`` / none), lib/core/function.py:98-104,140,158.
 
 Every op is a *member* (a pair of plain functions ``fwd``/``bwd`` taking a raw HIP stream);
-``GroupFn`` is the single autograd.Function.  A group runs its members CONCURRENTLY on forked
+``GroupFn`` is their autograd.Function (``LayerNormFn``: a layer norm by itself).  A group runs its members CONCURRENTLY on forked
 HIP streams and joins before returning: HRNet's 2-4 resolution branches, its fuse convs and
 the residual downsample paths are independent, and individually the low-resolution ones only
 launch 96-192 workgroups on a 256-CU chip.  All memory is allocated on the caller's stream
