@@ -164,11 +164,7 @@ class AdvmixHipError(RuntimeError):
 _ERR = {1: 'ADVMIX_EINVAL (bad argument / unsupported shape)', 2: 'ADVMIX_ELAUNCH (HIP runtime error)'}
 
 
-def failed(name, rc):
-    raise AdvmixHipError('%s failed: %s' % (name, _ERR.get(rc, rc)))
-
-
 def call(name, *args):
     rc = getattr(lib, name)(*args)
     if rc != 0:
-        failed(name, rc)
+        raise AdvmixHipError('%s failed: %s' % (name, _ERR.get(rc, rc)))

@@ -1,4 +1,4 @@
-"""Build libadvmix_hip.so (gfx950 only) with hipcc.  `python -m advmix_amd.build`."""
+"""Build libadvmix_hip.so (gfx950 only) with hipcc, and the torch-side module _node.so.  `python -m advmix_amd.build`."""
 import os
 import subprocess
 import sys
@@ -16,6 +16,22 @@ FLAGS = ['-O3', '--offload-arch=gfx950', '-fPIC', '-munsafe-fp-atomics', '-std=c
 # any, a spill is always an accident of a register cap, and spilling builds were among the suspects of round 3's
 # two-process NaN hunt (conv_direct.hip, at its launch bounds).  The compiler reports each kernel's scratch; the build reads it.
 RESOURCE_FLAG = '-Rpass-analysis=kernel-resource-usage'
+
+
+# The layer norm's autograd node: host code against torch's headers, a module of its own (the library knows no torch types).
+NODE, NODE_SO = 'layer_norm_node.cpp', os.path.join(HERE, '_node.so')
+
+
+def _node_command():
+    import sysconfig
+    import torch
+    inc = os.path.join(os.path.dirname(torch.__file__), 'include')
+    lib = os.path.join(os.path.dirname(torch.__file__), 'lib')
+    rocm = os.environ.get('ROCM_PATH', '/opt/rocm')
+    return [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+            '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch.compiled_with_cxx11_abi(), '-I' + inc, '-I' + os.path.join(inc, 'torch/csrc/api/include'),
+            '-I' + os.path.join(rocm, 'include'), '-I' + sysconfig.get_paths()['include'], os.path.join(CSRC, NODE), '-o', NODE_SO,
+            '-L' + lib, '-ltorch_python', '-ltorch_cpu', '-ltorch', '-lc10', '-lc10_hip', '-DADVMIX_TORCH="%s"' % torch.__version__]
 
 
 def _scratch_users(report):
@@ -62,9 +78,9 @@ def _stale_object(s, obj, src, hdrs, info):
     if not os.path.exists(obj):
         return True
     rec = info.get('objects', {}).get(s)
-    if rec and rec.get('headers_sha256_16') and rec.get('flags') is not None:
+    if rec and rec.get('headers_sha256_16') is not None and rec.get('flags') is not None:
         return (rec.get('source_sha256_16') != _sha(src) or rec['headers_sha256_16'] != {os.path.basename(h): _sha(h) for h in hdrs}
-                or rec['flags'] != FLAGS)
+                or rec['flags'] != (_node_command() if s == NODE else FLAGS))
     return _stale(obj, [src] + hdrs)
 
 
@@ -83,6 +99,11 @@ def build(force=False, verbose=True):
             if verbose:
                 print(' '.join(cmd), flush=True)
             procs.append((s, obj, subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True)))
+    if force or _stale_object(NODE, NODE_SO, os.path.join(CSRC, NODE), [], info):
+        cmd = _node_command()
+        if verbose:
+            print(' '.join(cmd), flush=True)
+        procs.append((NODE, NODE_SO, subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True)))
     bad = []
     for s, obj, p in procs:
         _, err = p.communicate()
@@ -93,7 +114,7 @@ def build(force=False, verbose=True):
             print('\n'.join(msgs), flush=True)
         if p.returncode != 0:
             sys.stderr.write(err[-4000:])
-            raise RuntimeError('hipcc failed on ' + s)
+            raise RuntimeError(('the C++ compiler' if s == NODE else 'hipcc') + ' failed on ' + s)
         users = _scratch_users(err)
         if users:
             os.remove(obj)                                  # never link it
@@ -102,7 +123,7 @@ def build(force=False, verbose=True):
         _record(hipcc, [s for s, obj, _ in procs if os.path.exists(obj)], False)      # what DID compile stays recorded
         raise RuntimeError('kernels with register spills / scratch are refused (see build.py):\n  ' + '\n  '.join(bad))
     linked = False
-    if force or procs or _stale(SO, objs):
+    if force or any(s != NODE for s, _, _ in procs) or _stale(SO, objs):
         cmd = [hipcc, '--offload-arch=gfx950', '-shared', '-fPIC', '-o', SO] + objs
         if verbose:
             print(' '.join(cmd), flush=True)
@@ -132,10 +153,11 @@ def _record(hipcc, compiled, linked):
     hdrs = {h: sha(os.path.join(HERE, *h.split('/'))) for h in ('csrc/common.h', '../include/advmix_hip.h')}
     for s in compiled:
         info['objects'][s] = {'source_sha256_16': sha(os.path.join(CSRC, s)), 'compiled_at': time.strftime('%Y-%m-%d %H:%M:%S'),
-                              'headers_sha256_16': {os.path.basename(h): v for h, v in hdrs.items()}, 'flags': FLAGS}
+                              'headers_sha256_16': {} if s == NODE else {os.path.basename(h): v for h, v in hdrs.items()},
+                              'flags': _node_command() if s == NODE else FLAGS}
     info.update({'last_call': {'at': time.strftime('%Y-%m-%d %H:%M:%S'), 'compiled': compiled, 'linked': linked},
                  'headers_sha256_16': hdrs, 'flags': FLAGS,
-                 'sources_now': {s: sha(os.path.join(CSRC, s)) for s in SOURCES},
+                 'sources_now': {s: sha(os.path.join(CSRC, s)) for s in SOURCES + [NODE]},
                  'library_sha256_16': sha(SO) if os.path.exists(SO) else None})
     info['up_to_date'] = all(info['objects'].get(s, {}).get('source_sha256_16') == h for s, h in info['sources_now'].items())
     try:

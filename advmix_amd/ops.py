@@ -10,7 +10,7 @@ them.  ``needs_input_grad`` carries the reference's three gradient modes (full /
 after ``set_require_grad(model, False)`` / none), lib/core/function.py:98-104,140,158.
 
 Every op is a *member* (a pair of plain functions ``fwd``/``bwd`` taking a raw HIP stream);
-``GroupFn`` is their autograd.Function (``LayerNormFn``: a layer norm by itself).  A group runs its members CONCURRENTLY on forked
+``GroupFn`` is their autograd.Function (a layer norm by itself has a node in C++, csrc/layer_norm_node.cpp).  A group runs its members CONCURRENTLY on forked
 HIP streams and joins before returning: HRNet's 2-4 resolution branches, its fuse convs and
 the residual downsample paths are independent, and individually the low-resolution ones only
 launch 96-192 workgroups on a 256-CU chip.  All memory is allocated on the caller's stream
@@ -21,7 +21,14 @@ import ctypes
 
 import torch
 
-from ._lib import call, failed, lib
+from ._lib import call, lib
+
+try:                                                       # the layer norm's autograd node (csrc/layer_norm_node.cpp): host code only,
+    from . import _node                                    # it calls the library's entry points by address
+except ImportError as e:
+    raise ImportError('advmix_amd: _node.so not found or not for this torch (%s) - build it with `python -m advmix_amd.build`' % e)
+_node.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.advmix_layer_norm_fwd, lib.advmix_layer_norm_bwd,
+                                                             lib.advmix_layer_norm_parts)))
 
 ACT_NONE, ACT_RELU, ACT_LEAKY = 0, 1, 2
 _CL = torch.channels_last
@@ -34,10 +41,6 @@ def _p(t):
 
 def _st():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-# the current stream's handle without a Stream object (0.2 instead of 2 us)
-_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 _KEEP = []      # temporaries created while a group's lanes are in flight; dropped after the join
@@ -1240,75 +1243,44 @@ class LayerNorm:
                 raise ValueError('layer_norm: %s requires a gradient but is not a leaf (parameter)' % name)
 
     @staticmethod
-    def launch(st, x, gamma, beta, eps, stats):
-        """(y, the fp32 [2, rows] means and rstds or None, (rows, C, distance of x's rows, type)); x: as LAYOUT leaves it, the
-        arguments checked."""
-        rows, C = LayerNorm._sizes(x)
-        y = LayerNorm._like(x)
-        s = torch.empty((2, rows), device=x.device, dtype=torch.float32) if stats else None
-        size = (rows, C, _row_stride(x), _LN_TYPES[x.dtype])
-        if rows:
-            at = None if s is None else s.data_ptr()
-            rc = lib.advmix_layer_norm_fwd(x.data_ptr(), size[2], None if gamma is None else gamma.data_ptr(),
-                                           None if beta is None else beta.data_ptr(), y.data_ptr(), at, at and at + 4 * rows, rows,
-                                           C, size[3], eps, st)
-            if rc:
-                failed('advmix_layer_norm_fwd', rc)
-        return y, s, size
-
-    @staticmethod
     def fwd(st, lane, t, meta, needs):
         x, gamma, beta = t
         x = LayerNorm.LAYOUT(x)
         LayerNorm.check(x, gamma, beta, meta)
-        y, s, size = LayerNorm.launch(st, x, gamma, beta, meta, any(needs))
-        return (y,), (() if s is None else (x, gamma, beta, s)), size
+        rows, C = LayerNorm._sizes(x)
+        y = LayerNorm._like(x)
+        mean = rstd = None
+        if any(needs):
+            mean, rstd = torch.empty((2, rows), device=x.device, dtype=torch.float32).unbind(0)
+        if rows:
+            call('advmix_layer_norm_fwd', _p(x), _row_stride(x), _p(gamma), _p(beta), _p(y), _p(mean), _p(rstd), rows, C,
+                 _LN_TYPES[x.dtype], meta, st)
+        return (y,), (() if mean is None else (x, gamma, beta, mean, rstd)), None
 
     @staticmethod
-    def bwd(st, lane, saved, size, meta, grads, needs, solo=False):
-        """``solo``: the launch is on the caller's stream and no other member runs beside it - a parameter's first gradient is
-        written instead of added to zeros, and temporaries need not outlive a join."""
+    def bwd(st, lane, saved, extra, meta, grads, needs):
         if torch.is_grad_enabled():
             raise RuntimeError('advmix_amd: layer_norm has no second derivative (backward with create_graph=True)')
-        x, gamma, beta, s = saved
-        rows, C, ldx, kind = size
-        dy = grads[0]
-        lddy = _row_stride(dy)
-        if lddy is None:
-            dy = LayerNorm._dense(dy)
-            lddy = _row_stride(dy)
-            if not solo:
-                keep(dy)
+        x, gamma, beta, mean, rstd = saved
+        dy = LayerNorm.LAYOUT(grads[0])
+        rows, C = LayerNorm._sizes(x)
         dx = LayerNorm._like(x) if needs[0] else None
-        dg, add_g = LayerNorm._grad(gamma, st, solo and rows) if needs[1] else (None, 0)
-        db, add_b = LayerNorm._grad(beta, st, solo and rows) if needs[2] else (None, 0)
+        dg = LayerNorm._grad(gamma, st) if needs[1] else None
+        db = LayerNorm._grad(beta, st) if needs[2] else None
         if rows:
-            part = None
+            kind, part = _LN_TYPES[x.dtype], None
             if dg is not None or db is not None:           # (this call's own: two captured graphs must not share it)
-                part = s.new_empty(lib.advmix_layer_norm_parts(rows, C, kind) * 2 * C)
-                if not solo:
-                    keep(part)
-            at = s.data_ptr()
-            rc = lib.advmix_layer_norm_bwd(dy.data_ptr(), lddy, x.data_ptr(), ldx, None if gamma is None else gamma.data_ptr(),
-                                           at, at + 4 * rows, None if dx is None else dx.data_ptr(),
-                                           None if dg is None else dg.data_ptr(), None if db is None else db.data_ptr(),
-                                           None if part is None else part.data_ptr(), add_g + 2 * add_b, rows, C, kind, st)
-            if rc:
-                failed('advmix_layer_norm_bwd', rc)
+                part = keep(torch.empty(lib.advmix_layer_norm_parts(rows, C, kind) * 2 * C, device=x.device, dtype=torch.float32))
+            call('advmix_layer_norm_bwd', _p(dy), _row_stride(dy), _p(x), _row_stride(x), _p(gamma), _p(mean), _p(rstd), _p(dx),
+                 _p(dg), _p(db), _p(part), 3, rows, C, kind, st)
         return dx, None, None
 
     @staticmethod
-    def _grad(p, st, write=False):
-        """(p.grad, 1 if the kernel has to add to it, 0 if it has to write it)."""
-        g = p.grad
-        if g is None:
-            if write and getattr(p, '_flat_grad_view', None) is None:
-                g = p.grad = torch.empty_like(p)
-                return g, 0
-            g = _grad_buf(p, st)
+    def _grad(p, st):
+        g = _grad_buf(p, st)
         if g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape or g.device != p.device:
             raise RuntimeError('layer_norm: a parameter\'s .grad must be a contiguous fp32 tensor of its shape')
-        return g, 1
+        return g
 
     @staticmethod
     def before_bwd(saved, needs, st):
@@ -1317,32 +1289,6 @@ class LayerNorm:
         for p, need in zip(saved[1:3], needs[1:3]):
             if need:
                 LayerNorm._grad(p, st)
-
-
-class LayerNormFn(torch.autograd.Function):
-    """A LayerNorm by itself: what GroupFn does for a group of one, without the lanes (host time of a small forward and backward
-    pass 96 us instead of 175 on one box, 51 instead of 91 on another).  gamma and beta are no inputs of the node - their gradients
-    go into .grad anyway: no nodes of theirs are run, and a capture does not meet what an eager graph of theirs left.  ``anchor``: a
-    leaf that keeps the node alive where x needs no gradient."""
-
-    @staticmethod
-    def forward(ctx, x, anchor, params, eps, wants):
-        gamma, beta = params
-        y, s, size = LayerNorm.launch(_raw_stream(x.device.index), x, gamma, beta, eps, True)
-        ctx.save_for_backward(x)
-        ctx.set_materialize_grads(False)
-        ctx.rest = (gamma, beta, s, size, wants, None if gamma is None else gamma._version)
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        if dy is None:
-            return None, None, None, None, None
-        gamma, beta, s, size, wants, version = ctx.rest
-        if gamma is not None and gamma._version != version:
-            raise RuntimeError('layer_norm: gamma was modified in place between the forward and the backward pass')
-        dx = LayerNorm.bwd(_raw_stream(dy.device.index), 0, ctx.saved_tensors + (gamma, beta, s), size, None, (dy,), wants, True)[0]
-        return dx, None, None, None, None
 
 
 class Act:
@@ -2026,19 +1972,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5):
     parameters' gradients are summed in fp32 in a fixed order; those gradients are accumulated into ``.grad`` as everywhere
     here.  No second derivative.  A backward pass may be captured into a HIP graph while an eager graph of the same gamma and
     beta is alive; with torch, not while one of the same leaf x is."""
-    LayerNorm.accept(x)
-    LayerNorm.check(x, gamma, beta, eps)
-    if x.device.index != torch.cuda.current_device():
-        with torch.cuda.device(x.device):
-            return layer_norm(x, gamma, beta, eps)
-    if _row_stride(x) is None:
-        x = LayerNorm._dense(x)                            # (a torch op: its own backward brings dx back into x's layout)
-    if torch.is_grad_enabled():
-        wants = (x.requires_grad, gamma is not None and gamma.requires_grad, beta is not None and beta.requires_grad)
-        if any(wants):
-            anchor = None if wants[0] else torch.empty(0, requires_grad=True)
-            return LayerNormFn.apply(x, anchor, (gamma, beta), eps, wants)
-    return LayerNorm.launch(_raw_stream(x.device.index), x, gamma, beta, eps, False)[0]
+    return _node.layer_norm(x, gamma, beta, eps, getattr(gamma, '_flat_grad_view', None), getattr(beta, '_flat_grad_view', None))
 
 
 def activation(x, act):

@@ -373,8 +373,7 @@ class FlatAdamW(FlatAdam):
         if not all(map(operator.is_, [p.grad for p in self._ps], self._grad_views)):      # (a step of 300 tensors: 10 us of this)
             super()._attach_grads(strict)
 
-    @torch.no_grad()
-    def step(self, closure=None, sync_hyper=True):
+    def step(self, closure=None, sync_hyper=True):           # (nothing in here is a torch op that autograd would see)
         self._ensure_flat()
         loss = None
         if closure is not None:

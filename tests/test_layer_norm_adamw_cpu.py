@@ -15,6 +15,12 @@ def test_layer_norm_refuses_the_cpu_and_other_types():
     for t in (torch.zeros(4, 8), torch.zeros(1, 8, 2, 2), torch.zeros(4, 8, dtype=torch.float64)):
         with pytest.raises(TypeError):
             ops.layer_norm(t)
+    x = torch.zeros(4, 8)
+    for bad in (('x',), (None,), (x, 1.0), (x, x, 'b'), (x, None, None, 'eps')):
+        with pytest.raises(TypeError):
+            ops.layer_norm(*bad)
+    with pytest.raises(TypeError):
+        ops._node.layer_norm(x)
 
 
 def test_row_stride_of_layouts():
