@@ -205,6 +205,11 @@ at::Tensor layer_norm(at::Tensor x, const at::Tensor& gamma, const at::Tensor& b
     return y;
 }
 
+struct WithoutGil {
+    PyThreadState* state = PyEval_SaveThread();
+    ~WithoutGil() { PyEval_RestoreThread(state); }
+};
+
 at::Tensor tensor_or_none(PyObject* o, const char* name) {
     if (o == Py_None) return at::Tensor();
     TORCH_CHECK_TYPE(THPVariable_Check(o), "layer_norm: ", name, " must be a tensor or None");
@@ -223,7 +228,7 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
                      fb = tensor_or_none(a[5], "gradient");
     at::Tensor x = THPVariable_Unpack(a[0]), y;
     {
-        const pybind11::gil_scoped_release free;
+        const WithoutGil free;                                   // (a launch may wait for room in a queue)
         y = layer_norm(std::move(x), gamma, beta, eps, fg, fb);
     }
     return THPVariable_Wrap(std::move(y));

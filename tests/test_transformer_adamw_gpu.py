@@ -479,9 +479,9 @@ def test_layer_norms_trained_with_adamw(bits):
 
 
 @pytest.mark.parametrize('bits,clip', [(32, None), (8, 1.0)])
-def test_advmix_step_as_graphs_and_eager(bits, clip):
-    """The AdvMix step with FlatAdamW for both networks, deterministic mode: three batches through AdvMixGraphRunner (warm-up,
-    snapshot, restore, replays) leave the bits that the eager step leaves."""
+def test_advmix_step_as_graphs_and_eager(bits, clip, monkeypatch):
+    """The AdvMix step with FlatAdamW for both networks, deterministic mode, one launch lane: three batches through
+    AdvMixGraphRunner (warm-up, snapshot, restore, replays) leave the bits that the eager step leaves."""
     import types
     from advmix_amd import ops
     from advmix_amd.core.function import advmix_step
@@ -489,6 +489,7 @@ def test_advmix_step_as_graphs_and_eager(bits, clip):
     from advmix_amd.utils.utils import adamw_groups
     from oracle.synth import synth_batch
     from test_models_gpu import _tiny_setup
+    monkeypatch.setattr(ops, 'MAX_LANES', 1)
     args = types.SimpleNamespace(alpha=0.1, adv_loss_weight=1.0)
     data = []
     for it in range(3):
