@@ -251,7 +251,8 @@ class FlatAdamW(FlatAdam):
     tensor (in memory order) with a power of two as their scale, rounded up or down by a hash of place, step and ``seed`` so that
     small steps count on average.  The same seed gives the same bits in every replica and after a resume.
     ``state_dict`` holds exp_avg / exp_avg_sq as torch.optim does, or with 8 bits exp_avg_codes / exp_avg_scale and
-    exp_avg_root_codes / exp_avg_root_scale as they are; either kind of optimizer loads either kind of state."""
+    exp_avg_root_codes / exp_avg_root_scale as they are; either kind of optimizer loads either kind of state.
+    A parameter that a loaded state lacks starts from zero moments; the step is one for all of them, the largest one loaded."""
 
     CHUNK, BLOCK, HYPER = 1024, 256, 8
 
@@ -424,10 +425,11 @@ class FlatAdamW(FlatAdam):
         sizes = [len(g['params']) for g in sd['param_groups']]
         if sizes != [len(g['params']) for g in self.param_groups]:
             raise ValueError('FlatAdamW: the state has other parameter groups (%r parameters)' % (sizes,))
-        todo = []
+        todo, fresh = [], []
         for i, p in enumerate(ps):                            # check everything before anything is overwritten
             st = sd['state'].get(i) or sd['state'].get(str(i))
             if st is None:
+                fresh.append((i, p))
                 continue
             lo, hi = self._blocks[i]
             for full, codes, scale in self._KEYS:
@@ -454,6 +456,11 @@ class FlatAdamW(FlatAdam):
         P = lambda t, at=0: ctypes.c_void_p(t.data_ptr() + at)          # noqa: E731
         with torch.no_grad(), torch.cuda.device(fp.device):
             st_ = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+            for i, p in fresh:                                # (saved before its first step)
+                for k in range(2):
+                    self._view(self._flat[2 + k], self._offsets[i], p).zero_()
+                    if self.state_bits == 8:
+                        self._scales[k][slice(*self._blocks[i])].zero_()
             other = [None, None]                              # the other width's image, made if the state needs it
             for i, p, st in todo:
                 off, (lo, hi), (c0, c1) = self._offsets[i], self._blocks[i], self._chunks[i]

@@ -227,6 +227,28 @@ def test_state_dict_round_trip_continues_bit_for_bit(bits, tmp_path):
     assert all(torch.equal(a, b) for a, b in zip(o.flat_state(), o2.flat_state()))
 
 
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_state_without_moments_starts_from_zero(bits):
+    def run(opt, ps, its):
+        for it in its:
+            opt.zero_grad()
+            for p, g in zip(ps, grads(ps, it)):
+                p.grad.copy_(g.to(dev()))
+            opt.step()
+    fresh, used = on_device(make()), on_device(make())
+    o1, o2 = AdamW(fresh, state_bits=bits), AdamW(used, state_bits=bits)
+    run(o2, used, range(3))
+    with torch.no_grad():
+        for a, b in zip(used, fresh):
+            a.copy_(b)
+    sd = torch.optim.AdamW(make()).state_dict()              # saved before its first step: no state at all
+    sd['param_groups'] = [{k: v for k, v in g.items() if k in ('lr', 'betas', 'eps', 'weight_decay', 'params')} for g in sd['param_groups']]
+    o2.load_state_dict(sd)
+    run(o1, fresh, range(3, 5))
+    run(o2, used, range(3, 5))
+    assert all(torch.equal(a, b) for a, b in zip(o1.flat_state(), o2.flat_state()))
+
+
 def test_state_of_the_other_width_and_of_torch():
     ref = [torch.nn.Parameter(p.detach().clone()) for p in make()]
     o_ref = torch.optim.AdamW(ref)
