@@ -68,7 +68,9 @@ void done(const char* name, int rc) {
 }
 
 struct Sizes {
-    int64_t rows, ldx;
+    at::DimVector of_x;
+    c10::Device device = c10::kCPU;
+    int64_t rows;
     int C, kind;
 };
 
@@ -108,6 +110,18 @@ struct LayerNormNode : torch::autograd::Node {
         x.reset_data();
         stats.reset();
     }
+    // t, read row by row: its layout is looked at here and now, since saved-tensor hooks may hand back x in another one (a copy
+    // of rows that lay apart is dense), or something that is not x at all.
+    struct Rows {
+        at::Tensor t;
+        int64_t ld;
+    };
+    Rows rows_of(const at::Tensor& t, const char* what) const {
+        TORCH_CHECK(t.sizes() == z.of_x && kind_of(t) == z.kind && t.device() == z.device, "layer_norm: ", what, " is ", t.scalar_type(), " ",
+                    t.sizes(), " on ", t.device(), ", not ", z.of_x, " of x's type on ", z.device);
+        const int64_t ld = row_stride(t);
+        return ld < 0 ? Rows{t.contiguous(format_of(t)), z.C} : Rows{t, ld};
+    }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         torch::autograd::variable_list out(num_outputs());
         if (!grads[0].defined()) return out;
@@ -116,14 +130,9 @@ struct LayerNormNode : torch::autograd::Node {
         const at::Tensor xs = x.unpack(shared_from_this());      // (refuses a second pass through a freed graph, and a changed x)
         TORCH_CHECK(!gamma.defined() || (int64_t)gamma._version() == version,
                     "layer_norm: gamma was modified in place between the forward and the backward pass");
-        at::Tensor dy = grads[0];
-        int64_t lddy = row_stride(dy);
-        if (lddy < 0) {
-            dy = dy.contiguous(format_of(dy));
-            lddy = channels(dy);
-        }
-        const c10::OptionalDeviceGuard guard(xs.device());
-        at::Tensor dx = want_x ? at::empty_like(xs, xs.options(), format_of(xs)) : at::Tensor();
+        const c10::OptionalDeviceGuard guard(z.device);
+        const Rows xr = rows_of(xs, "the saved x"), dr = rows_of(grads[0], "the gradient of y");
+        at::Tensor dx = want_x ? at::empty_like(xr.t, xr.t.options(), format_of(xr.t)) : at::Tensor();
         const Slot dg = want_gamma ? slot_of(gamma, flat_gamma, z.rows > 0) : Slot();
         const Slot db = want_beta ? slot_of(beta, flat_beta, z.rows > 0) : Slot();
         if (z.rows > 0) {
@@ -131,7 +140,7 @@ struct LayerNormNode : torch::autograd::Node {
             if (want_gamma || want_beta) part = at::empty({(int64_t)parts_entry(z.rows, z.C, z.kind) * 2 * z.C}, stats.options());
             const float* mean = stats.const_data_ptr<float>();
             done("advmix_layer_norm_bwd",
-                 bwd_entry(dy.const_data_ptr(), lddy, xs.const_data_ptr(), z.ldx, floats(gamma), mean, mean + z.rows,
+                 bwd_entry(dr.t.const_data_ptr(), dr.ld, xr.t.const_data_ptr(), xr.ld, floats(gamma), mean, mean + z.rows,
                            dx.defined() ? dx.mutable_data_ptr() : nullptr, dg.at(), db.at(),
                            part.defined() ? part.mutable_data_ptr<float>() : nullptr, (dg.add ? 1 : 0) + (db.add ? 2 : 0), z.rows, z.C,
                            z.kind, c10::hip::getCurrentHIPStream().stream()));
@@ -165,11 +174,13 @@ at::Tensor layer_norm(at::Tensor x, const at::Tensor& gamma, const at::Tensor& b
     check_param("gamma", gamma, x, C);
     check_param("beta", beta, x, C);
     const c10::OptionalDeviceGuard guard(x.device());
-    z.ldx = row_stride(x);
-    if (z.ldx < 0) {                                             // (a torch op: its own backward brings dx back into x's layout)
+    int64_t ldx = row_stride(x);
+    if (ldx < 0) {                                               // (a torch op: its own backward brings dx back into x's layout)
         x = x.contiguous(format_of(x));
-        z.ldx = C;
+        ldx = C;
     }
+    z.of_x = x.sizes();
+    z.device = x.device();
     z.C = (int)C;
     z.rows = x.numel() / C;
     const bool on = at::GradMode::is_enabled(), wx = on && x.requires_grad(), wg = on && gamma.defined() && gamma.requires_grad(),
@@ -182,7 +193,7 @@ at::Tensor layer_norm(at::Tensor x, const at::Tensor& gamma, const at::Tensor& b
     }
     if (z.rows > 0) {
         float* mean = keep ? stats.mutable_data_ptr<float>() : nullptr;
-        done("advmix_layer_norm_fwd", fwd_entry(x.const_data_ptr(), z.ldx, floats(gamma), floats(beta), y.mutable_data_ptr(), mean,
+        done("advmix_layer_norm_fwd", fwd_entry(x.const_data_ptr(), ldx, floats(gamma), floats(beta), y.mutable_data_ptr(), mean,
                                                 keep ? mean + z.rows : nullptr, z.rows, z.C, z.kind, (float)eps,
                                                 c10::hip::getCurrentHIPStream().stream()));
     }

@@ -1263,7 +1263,11 @@ class LayerNorm:
             raise RuntimeError('advmix_amd: layer_norm has no second derivative (backward with create_graph=True)')
         x, gamma, beta, mean, rstd = saved
         dy = LayerNorm.LAYOUT(grads[0])
+        x = LayerNorm.LAYOUT(x)                            # (saved-tensor hooks may hand it back in another layout, or as another tensor)
         rows, C = LayerNorm._sizes(x)
+        if x.shape != dy.shape or x.dtype != dy.dtype or x.device != dy.device or any(
+                s.shape != (rows,) or s.dtype != torch.float32 or s.device != x.device or not s.is_contiguous() for s in (mean, rstd)):
+            raise RuntimeError('layer_norm: the saved tensors are not those of the forward pass (saved-tensor hooks?)')
         dx = LayerNorm._like(x) if needs[0] else None
         dg = LayerNorm._grad(gamma, st) if needs[1] else None
         db = LayerNorm._grad(beta, st) if needs[2] else None
