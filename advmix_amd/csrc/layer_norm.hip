@@ -239,7 +239,7 @@ __global__ __launch_bounds__(threads_of(L)) void ln_fwd_kernel(const T* __restri
 // to[c] += v or = v
 __device__ __forceinline__ void give(float* to, int64_t c, float v, int add) {
     if (!to) return;
-    if (add) atomicAdd(to + c, v);                               // (one per element and launch: see ln_fold_kernel)
+    if (add) atomicAdd(to + c, v);                               // (one per sum and launch: see ln_fold_kernel)
     else to[c] = v;
 }
 
@@ -252,8 +252,8 @@ template <typename T, int L, int NV, bool TAIL, bool PAST>
 __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
                                                                  int64_t ldx, const float* __restrict__ gamma,
                                                                  const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                                 T* __restrict__ dx, float* __restrict__ dgamma,
-                                                                 float* __restrict__ dbeta, float* __restrict__ part, int add,
+                                                                 T* __restrict__ dx, float* dgamma, float* dbeta,
+                                                                 float* __restrict__ part, int add,
                                                                  int64_t rows, int C) {
     constexpr int V = Vec<T>::V, TH = L > 512 ? L : 512, R = TH / L, W = TH / 64;
     extern __shared__ float lds[];                               // row sums' box, then the workgroup's column sums [R waves][C]
@@ -396,11 +396,12 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
 }
 
 // The workgroups' partial sums in a fixed order: 16 columns x 64 slices of the partial rows per workgroup, so that a thread has at
-// most eight loads, all in flight (2.8 - 3 us, a launch's own time; 4.3 us for 4096 columns).  With ``add`` ONE atomic addition per element, so that two launches that share a gradient lose
-// neither's part.
+// most eight loads, all in flight (2.8 - 3 us, a launch's own time; 4.3 us for 4096 columns).  With ``add`` ONE atomic addition per
+// sum, so that two launches that add to one gradient (or one launch whose dgamma and dbeta are one) lose neither's part; a launch
+// that stores is for a gradient that no other one touches before it has run.
 constexpr int FOLD = 16;
-__global__ __launch_bounds__(1024) void ln_fold_kernel(const float* __restrict__ part, int parts, float* __restrict__ dgamma,
-                                                       float* __restrict__ dbeta, int add, int C) {
+__global__ __launch_bounds__(1024) void ln_fold_kernel(const float* __restrict__ part, int parts, float* dgamma, float* dbeta,
+                                                       int add, int C) {
     constexpr int S = 1024 / FOLD;
     __shared__ float box[FOLD][S + 1];
     const int j = threadIdx.x % FOLD, s = threadIdx.x / FOLD;

@@ -80,14 +80,15 @@ struct Slot {
     bool add = false;
     float* at() const { return grad.defined() ? grad.mutable_data_ptr<float>() : nullptr; }
 };
-// p.grad, made if there is none: the optimizer's flat view (added to, as the kernels everywhere here do) or a fresh tensor.
-Slot slot_of(const at::Tensor& p, const at::Tensor& flat, bool rows) {
+// p.grad, made if there is none: the optimizer's flat view (added to, as the kernels everywhere here do) or a fresh tensor, which
+// the kernel may store to (``store``) or has to find zeroed.
+Slot slot_of(const at::Tensor& p, const at::Tensor& flat, bool store) {
     Slot s;
     at::Tensor& g = p.mutable_grad();
     if (!g.defined() && flat.defined()) g = flat;
     if (!g.defined()) {
-        g = rows ? at::empty_like(p) : at::zeros_like(p);
-        s.add = !rows;
+        g = store ? at::empty_like(p) : at::zeros_like(p);
+        s.add = !store;
     } else {
         TORCH_CHECK(g.scalar_type() == at::kFloat && g.is_contiguous() && g.sizes() == p.sizes() && g.device() == p.device(),
                     "layer_norm: a parameter's .grad must be a contiguous fp32 tensor of its shape");
@@ -133,8 +134,9 @@ struct LayerNormNode : torch::autograd::Node {
         const c10::OptionalDeviceGuard guard(z.device);
         const Rows xr = rows_of(xs, "the saved x"), dr = rows_of(grads[0], "the gradient of y");
         at::Tensor dx = want_x ? at::empty_like(xr.t, xr.t.options(), format_of(xr.t)) : at::Tensor();
-        const Slot dg = want_gamma ? slot_of(gamma, flat_gamma, z.rows > 0) : Slot();
-        const Slot db = want_beta ? slot_of(beta, flat_beta, z.rows > 0) : Slot();
+        const bool store = z.rows > 0 && !(want_gamma && want_beta && gamma.is_same(beta));      // (one parameter as both: two sums in one place)
+        const Slot dg = want_gamma ? slot_of(gamma, flat_gamma, store) : Slot();
+        const Slot db = want_beta ? slot_of(beta, flat_beta, store) : Slot();
         if (z.rows > 0) {
             at::Tensor part;                                     // (this call's own: two captured graphs must not share it)
             if (want_gamma || want_beta) part = at::empty({(int64_t)parts_entry(z.rows, z.C, z.kind) * 2 * z.C}, stats.options());

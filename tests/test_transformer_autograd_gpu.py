@@ -3,7 +3,7 @@ tolerances are those of the layer norm's own tests."""
 import pytest
 import torch
 
-from test_transformer_layer_norm_gpu import check_grads, check_y, dev, formula, inputs, ops
+from test_transformer_layer_norm_gpu import U, check, check_grads, check_y, dev, formula, inputs, ops
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,23 @@ def test_saved_x_that_is_not_x_is_refused(how, form):
         y.backward(dy)
     norm(form, x, gamma, beta).backward(dy)
     check_grads(x.grad, None, None, formula(x, gamma, beta, dy, 1e-5))
+
+
+@pytest.mark.parametrize('form', ['single', 'group'])
+@pytest.mark.parametrize('shape', [(0, 16), (1, 16), (3, 2), (16, 768), (700, 100), (900, 3), (3, 16384), (2, 20000), (2, 24, 6, 5)], ids=str)
+def test_one_parameter_as_gamma_and_beta(shape, form):
+    """Its gradient is the sum of both, whether it has one yet or not."""
+    x, dy, p, _ = inputs(shape, torch.float32)
+    f = formula(x, p, p, dy, 1e-5)
+    both = dict(f, both=f['dg'] + f['db'])
+    for times in (1, 2):
+        y = norm(form, x, p, p)
+        y.backward(dy)
+        if not f['dy'].numel():
+            assert not p.grad.any()
+            continue
+        check_y(y, f)
+        rows, C = f['xh'].shape
+        e = (C / 64 + 16) * (f['R'] + 2) + 8
+        tol = (rows / 256 + 512 + 4) * U * ((f['dy'] * f['xh']).abs().sum(0) + f['dy'].abs().sum(0)) + (e * U * (1 + f['xh'].abs()) * f['dy'].abs()).sum(0)
+        check('dgamma + dbeta', p.grad, times * both['both'], times * tol)
