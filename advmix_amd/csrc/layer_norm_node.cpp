@@ -74,6 +74,40 @@ struct Sizes {
     int C, kind;
 };
 
+// gamma and beta are no inputs of the node, so the engine does not order the passes that write their gradients.  A gradient that is
+// made in a pass holds nothing until that pass's first write has run: it carries the stream of that write (with the tensor itself,
+// as its backend meta), and whoever adds to it on another stream lets that one wait first.
+struct FirstWrite : c10::BackendMeta {
+    c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream();
+};
+void first_written_here(const at::Tensor& grad) {
+    grad.unsafeGetTensorImpl()->set_backend_meta(c10::make_intrusive<FirstWrite>());
+}
+// The graph capture that a stream takes part in, if any (the null stream takes part in none, and may not be asked during one).
+struct Capture {
+    bool active = false;
+    unsigned long long id = 0;
+    explicit Capture(hipStream_t s) {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (s != nullptr && hipStreamGetCaptureInfo(s, &status, &id) == hipSuccess) active = status == hipStreamCaptureStatusActive;
+    }
+};
+void wait_for_first_write(const at::Tensor& grad) {
+    const auto* first = dynamic_cast<const FirstWrite*>(grad.unsafeGetTensorImpl()->get_backend_meta());
+    if (!first) return;
+    const hipStream_t mine = c10::hip::getCurrentHIPStream().stream(), its = first->stream.stream();
+    if (mine == its) return;
+    const Capture a(mine), b(its);                               // (work of a capture and work outside it cannot wait for each other)
+    if (a.active != b.active || (a.active && a.id != b.id)) return;
+    hipEvent_t event;
+    bool ok = hipEventCreateWithFlags(&event, hipEventDisableTiming) == hipSuccess;
+    if (ok) {
+        ok = hipEventRecord(event, its) == hipSuccess && hipStreamWaitEvent(mine, event, 0) == hipSuccess;
+        ok = hipEventDestroy(event) == hipSuccess && ok;
+    }
+    TORCH_CHECK(ok, "layer_norm: could not order a parameter's gradient between streams (HIP runtime error)");
+}
+
 // One gradient of gamma or beta: where the kernel puts it, and whether it adds.
 struct Slot {
     at::Tensor grad;
@@ -88,10 +122,12 @@ Slot slot_of(const at::Tensor& p, const at::Tensor& flat, bool store) {
     if (!g.defined() && flat.defined()) g = flat;
     if (!g.defined()) {
         g = store ? at::empty_like(p) : at::zeros_like(p);
+        first_written_here(g);
         s.add = !store;
     } else {
         TORCH_CHECK(g.scalar_type() == at::kFloat && g.is_contiguous() && g.sizes() == p.sizes() && g.device() == p.device(),
                     "layer_norm: a parameter's .grad must be a contiguous fp32 tensor of its shape");
+        wait_for_first_write(g);
         s.add = true;
     }
     s.grad = g;
@@ -248,6 +284,17 @@ PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// first_written_here(t), wait_for_first_write(t): for gradients that the launch groups' member makes and adds to
+template <void (*F)(const at::Tensor&)> PyObject* py_grad(PyObject*, PyObject* t) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(THPVariable_Check(t), "expected a tensor");
+    const at::Tensor& grad = THPVariable_Unpack(t);
+    const c10::OptionalDeviceGuard guard(grad.device());
+    F(grad);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(address of advmix_layer_norm_fwd, of _bwd, of _parts)
 PyObject* py_bind(PyObject*, PyObject* args) {
     unsigned long long f = 0, b = 0, p = 0;
@@ -259,6 +306,8 @@ PyObject* py_bind(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {{"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_layer_norm)), METH_FASTCALL, nullptr},
+                         {"first_written_here", py_grad<first_written_here>, METH_O, nullptr},
+                         {"wait_for_first_write", py_grad<wait_for_first_write>, METH_O, nullptr},
                          {"bind", py_bind, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_node", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1281,7 +1281,9 @@ class LayerNorm:
 
     @staticmethod
     def _grad(p, st):
+        fresh = p.grad is None and getattr(p, '_flat_grad_view', None) is None
         g = _grad_buf(p, st)
+        (_node.first_written_here if fresh else _node.wait_for_first_write)(g)      # (a layer norm by itself may run on another stream)
         if g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape or g.device != p.device:
             raise RuntimeError('layer_norm: a parameter\'s .grad must be a contiguous fp32 tensor of its shape')
         return g

@@ -68,6 +68,19 @@ def test_saved_x_that_is_not_x_is_refused(how, form):
     check_grads(x.grad, None, None, formula(x, gamma, beta, dy, 1e-5))
 
 
+def check_sum(got, parts, what):
+    """A gradient that several sums meet in: (sum, its terms' magnitudes, rows, e of the formula's tolerance) each, and a rounding of
+    the total for every addition."""
+    want = sum(f[what] for f in parts)
+    tol = 0
+    for f in parts:
+        (rows, C), n = f['xh'].shape, f['xh'].shape[1] / 64 + 16
+        e = (n * (f['R'] + 2) + 8) * U * (1 + f['xh'].abs())
+        terms = f['dy'] * f['xh'] if what == 'dg' else f['dy']
+        tol = tol + (rows / 256 + 512 + len(parts)) * U * terms.abs().sum(0) + ((e * f['dy'].abs()).sum(0) if what == 'dg' else 0)
+    check(what, got, want, tol)
+
+
 @pytest.mark.parametrize('form', ['single', 'group'])
 @pytest.mark.parametrize('shape', [(0, 16), (1, 16), (3, 2), (16, 768), (700, 100), (900, 3), (3, 16384), (2, 20000), (2, 24, 6, 5)], ids=str)
 def test_one_parameter_as_gamma_and_beta(shape, form):
@@ -86,3 +99,79 @@ def test_one_parameter_as_gamma_and_beta(shape, form):
         e = (C / 64 + 16) * (f['R'] + 2) + 8
         tol = (rows / 256 + 512 + 4) * U * ((f['dy'] * f['xh']).abs().sum(0) + f['dy'].abs().sum(0)) + (e * U * (1 + f['xh'].abs()) * f['dy'].abs()).sum(0)
         check('dgamma + dbeta', p.grad, times * both['both'], times * tol)
+
+
+def two_streams(forms, wait):
+    """Two layer norms with the same gamma and beta, none of them with a gradient yet, forward on two streams, backward in one pass;
+    the stream of the node that runs first is busy, so its first write comes last if nothing waits for it."""
+    one = inputs((400, 72), torch.float32)
+    two = inputs((300, 72), torch.float32, seed=9)
+    gamma, beta = one[2:]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ys = []
+    for (x, dy, _, _), s, form in zip((one, two), streams, forms):
+        x.requires_grad_()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            ys.append(norm(form, x, gamma, beta))
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    with torch.cuda.stream(streams[1]):                     # (the later node runs first)
+        torch.cuda._sleep(wait)
+    torch.autograd.backward(ys, [one[1], two[1]])
+    for s in streams:
+        torch.cuda.current_stream().wait_stream(s)
+    fs = [formula(x, gamma, beta, dy, 1e-5) for x, dy, _, _ in (one, two)]
+    for (x, _, _, _), f in zip((one, two), fs):
+        check_grads(x.grad, None, None, f)
+    check_sum(gamma.grad, fs, 'dg')
+    check_sum(beta.grad, fs, 'db')
+
+
+@pytest.mark.parametrize('forms', [('single', 'single'), ('group', 'single'), ('single', 'group')], ids=str)
+def test_shared_parameters_on_two_streams(forms):
+    two_streams(forms, 20000000)
+
+
+def test_shared_parameters_on_two_streams_of_a_capture():
+    """The same inside one captured graph: every replay leaves the eager sum."""
+    o = ops()
+    one, two = inputs((400, 72), torch.float32), inputs((300, 72), torch.float32, seed=9)
+    gamma, beta = one[2:]
+    leaves = [t[0].clone().requires_grad_() for t in (one, two)]
+    other = torch.cuda.Stream()
+
+    def both():
+        cur = torch.cuda.current_stream()
+        other.wait_stream(cur)
+        y1 = o.layer_norm(leaves[0], gamma, beta)
+        with torch.cuda.stream(other):
+            y2 = o.layer_norm(leaves[1], gamma, beta)
+        cur.wait_stream(other)
+        torch.autograd.backward([y1, y2], [one[1], two[1]])
+        cur.wait_stream(other)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    want = [p.grad.clone() for p in (gamma, beta)]
+    fs = [formula(t[0], gamma, beta, t[1], 1e-5) for t in (one, two)]
+    check_sum(want[0], fs, 'dg')
+    check_sum(want[1], fs, 'db')
+    for t in (*leaves, gamma, beta):
+        t.grad = None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        both()
+    made = [gamma.grad, beta.grad]
+    for _ in range(4):
+        for t in made:
+            t.fill_(float('nan'))                           # (made in the capture: the first pass stores)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(made, want))
+    o.layer_norm(leaves[0], gamma, beta).backward(one[1])   # an eager pass on another stream than the capture's adds to them
+    check_sum(gamma.grad, fs + fs[:1], 'dg')
+    check_sum(beta.grad, fs + fs[:1], 'db')
