@@ -8,12 +8,14 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 namespace {
 
@@ -62,6 +64,11 @@ int kind_of(const at::Tensor& t) {
 }
 
 const float* floats(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+
+// Forward mode: a tangent would be dropped without a word, the result taken for a constant.
+void refuse_tangent(const char* name, const at::Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "layer_norm: no forward-mode derivatives, and ", name, " has a tangent");
+}
 
 void done(const char* name, int rc) {
     TORCH_CHECK(rc == 0, name, " failed: ", rc == 1 ? "ADVMIX_EINVAL (bad argument / unsupported shape)" : "ADVMIX_ELAUNCH (HIP runtime error)");
@@ -168,6 +175,8 @@ struct LayerNormNode : torch::autograd::Node {
         TORCH_CHECK(!gamma.defined() || (int64_t)gamma._version() == version,
                     "layer_norm: gamma was modified in place between the forward and the backward pass");
         const c10::OptionalDeviceGuard guard(z.device);
+        refuse_tangent("the saved x", xs);
+        refuse_tangent("the gradient of y", grads[0]);
         const Rows xr = rows_of(xs, "the saved x"), dr = rows_of(grads[0], "the gradient of y");
         at::Tensor dx = want_x ? at::empty_like(xr.t, xr.t.options(), format_of(xr.t)) : at::Tensor();
         const bool store = z.rows > 0 && !(want_gamma && want_beta && gamma.is_same(beta));      // (one parameter as both: two sums in one place)
@@ -199,6 +208,9 @@ void check_param(const char* name, const at::Tensor& p, const at::Tensor& x, int
 
 at::Tensor layer_norm(at::Tensor x, const at::Tensor& gamma, const at::Tensor& beta, double eps, const at::Tensor& flat_gamma,
                       const at::Tensor& flat_beta) {
+    refuse_tangent("x", x);
+    refuse_tangent("gamma", gamma);
+    refuse_tangent("beta", beta);
     Sizes z;
     z.kind = kind_of(x);
     TORCH_CHECK_TYPE(z.kind >= 0 && x.is_cuda(), "layer_norm needs fp32, bf16 or fp16 CUDA tensors (no CPU fallback), got ",

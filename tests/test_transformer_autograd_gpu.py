@@ -175,3 +175,16 @@ def test_shared_parameters_on_two_streams_of_a_capture():
     o.layer_norm(leaves[0], gamma, beta).backward(one[1])   # an eager pass on another stream than the capture's adds to them
     check_sum(gamma.grad, fs + fs[:1], 'dg')
     check_sum(beta.grad, fs + fs[:1], 'db')
+
+
+def test_forward_mode_through_the_backward_pass_is_refused():
+    """A gradient with a tangent: its derivative would be dropped.  The graph stays as it is."""
+    import torch.autograd.forward_ad as fwd_ad
+    x, dy, gamma, beta = inputs((20, 24), torch.float32)
+    y = ops().layer_norm(x.requires_grad_(), gamma, beta)
+    with fwd_ad.dual_level():
+        with pytest.raises(NotImplementedError, match='tangent'):
+            torch.autograd.grad(y, x, fwd_ad.make_dual(dy, torch.ones_like(dy)))
+    assert gamma.grad is None
+    y.backward(dy)
+    check_grads(x.grad, gamma.grad, beta.grad, formula(x, gamma, beta, dy, 1e-5))
