@@ -65,6 +65,16 @@ int kind_of(const at::Tensor& t) {
 
 const float* floats(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 
+// What records operations in order to run them again sees the output's allocation and nothing of the kernels that fill it.
+void refuse_recording() {
+    using Key = c10::impl::TorchDispatchModeKey;
+    const auto mode = [](Key k) { return c10::impl::TorchDispatchModeTLS::get_mode(k).has_value(); };
+    const auto included = [](c10::DispatchKey k) { return c10::impl::tls_is_dispatch_key_included(k); };
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !mode(Key::PROXY) && !mode(Key::FAKE) && !mode(Key::FUNCTIONAL) &&
+                                    !included(c10::DispatchKey::PreDispatch) && !included(c10::DispatchKey::Functionalize) &&
+                                    !included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode),
+                                "layer_norm: its kernels cannot be recorded (torch.jit.trace, make_fx, fake tensors) or transformed (torch.func)");
+}
 // Forward mode: a tangent would be dropped without a word, the result taken for a constant.
 void refuse_tangent(const char* name, const at::Tensor& t) {
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "layer_norm: no forward-mode derivatives, and ", name, " has a tangent");
@@ -175,6 +185,7 @@ struct LayerNormNode : torch::autograd::Node {
         TORCH_CHECK(!gamma.defined() || (int64_t)gamma._version() == version,
                     "layer_norm: gamma was modified in place between the forward and the backward pass");
         const c10::OptionalDeviceGuard guard(z.device);
+        refuse_recording();
         refuse_tangent("the saved x", xs);
         refuse_tangent("the gradient of y", grads[0]);
         const Rows xr = rows_of(xs, "the saved x"), dr = rows_of(grads[0], "the gradient of y");
@@ -208,6 +219,7 @@ void check_param(const char* name, const at::Tensor& p, const at::Tensor& x, int
 
 at::Tensor layer_norm(at::Tensor x, const at::Tensor& gamma, const at::Tensor& beta, double eps, const at::Tensor& flat_gamma,
                       const at::Tensor& flat_beta) {
+    refuse_recording();
     refuse_tangent("x", x);
     refuse_tangent("gamma", gamma);
     refuse_tangent("beta", beta);

@@ -24,3 +24,44 @@ def test_forward_mode(which):
             ops.layer_norm(*args())
     with pytest.raises(TypeError):
         ops.layer_norm(*a)                                  # the level is closed
+
+
+def traced(f, x):
+    torch.jit.trace(f, (x,), check_trace=False)
+
+
+def symbolic(**how):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    return lambda f, x: make_fx(f, **how)(x)
+
+
+def fake(f, x):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        f(torch.randn(5, 8))
+
+
+RECORDERS = {'jit.trace': traced, 'make_fx': symbolic(), 'make_fx, pre-dispatch': symbolic(pre_dispatch=True),
+             'make_fx, fake': symbolic(tracing_mode='fake'), 'make_fx, symbolic': symbolic(tracing_mode='symbolic'), 'fake tensors': fake,
+             'functionalize': lambda f, x: torch.func.functionalize(f)(x), 'func.grad': lambda f, x: torch.func.grad(lambda v: f(v).sum())(x),
+             'func.vjp': lambda f, x: torch.func.vjp(f, x), 'vmap': lambda f, x: torch.func.vmap(f)(x)}
+
+
+@pytest.mark.parametrize('of', ['its input', 'another input'])
+@pytest.mark.parametrize('how', list(RECORDERS))
+def test_recording(how, of):
+    """A recorded graph would hold the output's allocation and none of the kernels."""
+    c = torch.randn(5, 8)
+    f = (lambda v: ops.layer_norm(v) * 1) if of == 'its input' else (lambda v: v * ops.layer_norm(c))
+    with pytest.raises(NotImplementedError, match='record'):
+        RECORDERS[how](f, torch.randn(5, 8))
+    with pytest.raises(TypeError):                          # none is active any more: the device is what is wrong
+        f(torch.randn(5, 8))
+
+
+def test_what_only_watches_operations_is_not_refused():
+    """Modes that count or hand on what runs do not make the result wrong: the device is what is wrong here."""
+    from torch.utils.flop_counter import FlopCounterMode
+    with FlopCounterMode(display=False), torch.device('cpu'):
+        with pytest.raises(TypeError):
+            ops.layer_norm(torch.randn(5, 8))

@@ -188,3 +188,39 @@ def test_forward_mode_through_the_backward_pass_is_refused():
     assert gamma.grad is None
     y.backward(dy)
     check_grads(x.grad, gamma.grad, beta.grad, formula(x, gamma, beta, dy, 1e-5))
+
+
+@pytest.mark.parametrize('how', ['jit.trace', 'make_fx'])
+def test_recording_is_refused(how):
+    """A recorded graph would hold the allocation of y (of dx) and none of the kernels."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    record = (lambda f, t: torch.jit.trace(f, (t,), check_trace=False)) if how == 'jit.trace' else lambda f, t: make_fx(f)(t)
+    x, dy, gamma, beta = inputs((20, 24), torch.float32)
+    with pytest.raises(NotImplementedError, match='record'):
+        record(lambda t: ops().layer_norm(t, gamma, beta) * 1, x)
+    y = ops().layer_norm(x.requires_grad_(), gamma, beta)
+    if how == 'make_fx':                                    # (a trace runs the backward pass as a whole)
+        with pytest.raises(NotImplementedError, match='record'):
+            record(lambda g: torch.autograd.grad(y, x, g, retain_graph=True)[0], dy)
+        assert gamma.grad is None
+    y.backward(dy)
+    check_grads(x.grad, gamma.grad, beta.grad, formula(x, gamma, beta, dy, 1e-5))
+
+
+def test_checkpointed_compiled_and_counted():
+    """What runs the layer norm as it is keeps running it: checkpoints of both kinds, a compiled function around it, a counting mode."""
+    from torch.utils.checkpoint import checkpoint
+    from torch.utils.flop_counter import FlopCounterMode
+    x, dy, gamma, beta = inputs((20, 24), torch.float32)
+    f = formula(x, gamma, beta, dy, 1e-5)
+    x.requires_grad_()
+    plain = lambda t: ops().layer_norm(t, gamma, beta)          # noqa: E731
+    for run in (lambda t: checkpoint(plain, t, use_reentrant=True), lambda t: checkpoint(plain, t, use_reentrant=False),
+                torch.compile(plain, backend='eager')):
+        x.grad = gamma.grad = beta.grad = None
+        y = run(x)
+        check_y(y, f)
+        y.backward(dy)
+        check_grads(x.grad, gamma.grad, beta.grad, f)
+    with FlopCounterMode(display=False), torch.no_grad():
+        check_y(plain(x), f)
