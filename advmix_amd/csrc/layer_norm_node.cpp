@@ -75,6 +75,17 @@ void refuse_recording() {
                                     !included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode),
                                 "layer_norm: its kernels cannot be recorded (torch.jit.trace, make_fx, fake tensors) or transformed (torch.func)");
 }
+// A tensor whose values are what its memory holds, by strides: no wrapper (subclasses with a dispatch of their own, torch.func's,
+// batched gradients), no sparse or nested one.  ``values`` then makes memory of two views that hold none or other values.
+bool plain(const at::Tensor& t) {
+    static const c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::Batched,
+                                               c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper});
+    return t.layout() == at::kStrided && !t.is_nested() && !t.key_set().has_any(wrappers);
+}
+at::Tensor values(const at::Tensor& t) {
+    if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+    return t.is_neg() ? t.resolve_neg() : t;
+}
 // Forward mode: a tangent would be dropped without a word, the result taken for a constant.
 void refuse_tangent(const char* name, const at::Tensor& t) {
     TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "layer_norm: no forward-mode derivatives, and ", name, " has a tangent");
@@ -171,10 +182,12 @@ struct LayerNormNode : torch::autograd::Node {
         int64_t ld;
     };
     Rows rows_of(const at::Tensor& t, const char* what) const {
+        TORCH_CHECK(plain(t), "layer_norm: ", what, " is no plain tensor");
         TORCH_CHECK(t.sizes() == z.of_x && kind_of(t) == z.kind && t.device() == z.device, "layer_norm: ", what, " is ", t.scalar_type(), " ",
                     t.sizes(), " on ", t.device(), ", not ", z.of_x, " of x's type on ", z.device);
-        const int64_t ld = row_stride(t);
-        return ld < 0 ? Rows{t.contiguous(format_of(t)), z.C} : Rows{t, ld};
+        const at::Tensor v = values(t);
+        const int64_t ld = row_stride(v);
+        return ld < 0 ? Rows{v.contiguous(format_of(v)), z.C} : Rows{v, ld};
     }
     torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
         torch::autograd::variable_list out(num_outputs());
@@ -210,6 +223,7 @@ struct LayerNormNode : torch::autograd::Node {
 
 void check_param(const char* name, const at::Tensor& p, const at::Tensor& x, int64_t C) {
     if (!p.defined()) return;
+    TORCH_CHECK_TYPE(plain(p) && !p.is_neg() && !p._is_zerotensor(), "layer_norm: ", name, " must be a plain tensor");
     TORCH_CHECK_TYPE(p.scalar_type() == at::kFloat && p.device() == x.device(), "layer_norm: ", name, " must be fp32 on ", x.device(),
                      ", got ", p.scalar_type(), " on ", p.device());
     TORCH_CHECK_VALUE(p.dim() == 1 && p.size(0) == C && p.is_contiguous(), "layer_norm: ", name, " must be a contiguous [", C, "], got ",
@@ -227,6 +241,7 @@ at::Tensor layer_norm(at::Tensor x, const at::Tensor& gamma, const at::Tensor& b
     z.kind = kind_of(x);
     TORCH_CHECK_TYPE(z.kind >= 0 && x.is_cuda(), "layer_norm needs fp32, bf16 or fp16 CUDA tensors (no CPU fallback), got ",
                      x.scalar_type(), " on ", x.device());
+    TORCH_CHECK_TYPE(plain(x) && !x._is_zerotensor(), "layer_norm: x must be a plain tensor");
     TORCH_CHECK_VALUE(x.dim() >= 1 && x.dim() <= 4, "layer_norm: expected tokens [..., C] with up to 3 dimensions or a 4-D NCHW map, got ",
                       x.dim(), "-D");
     const int64_t C = channels(x);
@@ -236,6 +251,7 @@ at::Tensor layer_norm(at::Tensor x, const at::Tensor& gamma, const at::Tensor& b
     check_param("gamma", gamma, x, C);
     check_param("beta", beta, x, C);
     const c10::OptionalDeviceGuard guard(x.device());
+    x = values(x);
     int64_t ldx = row_stride(x);
     if (ldx < 0) {                                               // (a torch op: its own backward brings dx back into x's layout)
         x = x.contiguous(format_of(x));

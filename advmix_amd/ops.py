@@ -1201,15 +1201,20 @@ class LayerNorm:
 
     @staticmethod
     def accept(t):
-        if t.dtype not in _LN_TYPES or not t.is_cuda:
+        if t.dtype not in _LN_TYPES or not t.is_cuda or t.layout != torch.strided or t.is_nested:
             raise TypeError('layer_norm needs fp32, bf16 or fp16 CUDA tensors (no CPU fallback), got %s on %s' % (t.dtype, t.device))
         if not 1 <= t.dim() <= 4:
             raise ValueError('layer_norm: expected tokens [..., C] with up to 3 dimensions or a 4-D NCHW map, got %d-D' % t.dim())
 
     @staticmethod
     def LAYOUT(t):
-        """What GroupFn does to x and to dy BEFORE the lanes fork: checks, and a dense copy if the rows do not line up."""
+        """What GroupFn does to x and to dy BEFORE the lanes fork: checks, memory for views that have none of their own or that
+        count with the other sign, and a dense copy if the rows do not line up."""
         LayerNorm.accept(t)
+        if t._is_zerotensor():
+            t = keep(torch.zeros(t.shape, dtype=t.dtype, device=t.device))
+        elif t.is_neg():
+            t = keep(t.resolve_neg())
         return t if _row_stride(t) is not None else keep(LayerNorm._dense(t))
 
     @staticmethod
@@ -1235,6 +1240,8 @@ class LayerNorm:
         for name, p in (('gamma', gamma), ('beta', beta)):
             if p is None:
                 continue
+            if p.layout != torch.strided or p.is_neg() or p._is_zerotensor():
+                raise TypeError('layer_norm: %s must be a plain tensor' % name)
             if p.dtype != torch.float32 or p.device != x.device:
                 raise TypeError('layer_norm: %s must be fp32 on %s, got %s on %s' % (name, x.device, p.dtype, p.device))
             if p.shape != (C,) or not p.is_contiguous():

@@ -224,3 +224,52 @@ def test_checkpointed_compiled_and_counted():
         check_grads(x.grad, gamma.grad, beta.grad, f)
     with FlopCounterMode(display=False), torch.no_grad():
         check_y(plain(x), f)
+
+
+@pytest.mark.parametrize('form', ['single', 'group'])
+def test_views_of_the_other_sign_and_zeros_without_memory(form):
+    """x and dy as lazy negatives, dy as torch's zeros that own no memory: what they stand for counts."""
+    x, dy, gamma, beta = inputs((20, 24), torch.float32)
+    xn = x.clone().requires_grad_()
+    y = norm(form, xn._neg_view(), gamma, beta)
+    f = formula(-x, gamma, beta, -dy, 1e-5)
+    check_y(y, f)
+    y.backward(dy._neg_view(), retain_graph=True)
+    check_grads(-xn.grad, gamma.grad, beta.grad, f)
+    xn.grad = gamma.grad = beta.grad = None
+    y.backward(torch._efficientzerotensor(20, 24, device=dev()))
+    assert not xn.grad.any() and not gamma.grad.any() and not beta.grad.any()
+    x, dy, gamma, beta = inputs((20, 1), torch.float32)      # (one channel: any stride would do)
+    norm(form, x.requires_grad_(), gamma, beta).backward(torch._efficientzerotensor(20, 1, device=dev()))
+    assert not x.grad.any() and not gamma.grad.any() and not beta.grad.any()
+
+
+class Wrapped(torch.Tensor):
+    """A tensor whose operations are Python's, without memory of its own."""
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, f, types, a=(), k=None):
+        raise AssertionError('no operation of this tensor is to run')
+
+
+def test_what_is_no_plain_tensor_is_refused():
+    """Checked on the host, before any launch."""
+    o = ops()
+    x, dy, gamma, beta = inputs((20, 24), torch.float32)
+    for bad in (x.to_sparse(), Wrapped(x), torch._efficientzerotensor(20, 24, device=dev())):
+        with pytest.raises(TypeError):
+            o.layer_norm(bad, gamma, beta)
+    for bad in (gamma.detach()._neg_view(), Wrapped(gamma), torch._efficientzerotensor(24, device=dev()), gamma.detach().to_sparse()):
+        for form in ('single', 'group') if type(bad) is torch.Tensor else ('single',):
+            with pytest.raises(TypeError):
+                norm(form, x, bad, beta)
+            with pytest.raises(TypeError):
+                norm(form, x, gamma, bad)
+    y = o.layer_norm(x.requires_grad_(), gamma, beta)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.autograd.grad(y, x, torch.stack([dy, dy]), is_grads_batched=True, retain_graph=True)
+    y.backward(dy)
+    check_grads(x.grad, gamma.grad, beta.grad, formula(x, gamma, beta, dy, 1e-5))
