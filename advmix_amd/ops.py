@@ -1262,13 +1262,17 @@ class LayerNorm:
         if rows:
             call('advmix_layer_norm_fwd', _p(x), _row_stride(x), _p(gamma), _p(beta), _p(y), _p(mean), _p(rstd), rows, C,
                  _LN_TYPES[x.dtype], meta, st)
-        return (y,), (() if mean is None else (x, gamma, beta, mean, rstd)), None
+        # gamma and beta are kept as they are, not as saved tensors: saved-tensor hooks hand back copies, whose .grad nobody reads
+        return (y,), (() if mean is None else (x, mean, rstd)), (gamma, beta, 0 if gamma is None else gamma._version)
 
     @staticmethod
     def bwd(st, lane, saved, extra, meta, grads, needs):
         if torch.is_grad_enabled():
             raise RuntimeError('advmix_amd: layer_norm has no second derivative (backward with create_graph=True)')
-        x, gamma, beta, mean, rstd = saved
+        x, mean, rstd = saved
+        gamma, beta, version = extra
+        if gamma is not None and gamma._version != version:
+            raise RuntimeError('layer_norm: gamma was modified in place between the forward and the backward pass')
         dy = LayerNorm.LAYOUT(grads[0])
         x = LayerNorm.LAYOUT(x)                            # (saved-tensor hooks may hand it back in another layout, or as another tensor)
         rows, C = LayerNorm._sizes(x)
@@ -1296,10 +1300,10 @@ class LayerNorm:
         return g
 
     @staticmethod
-    def before_bwd(saved, needs, st):
+    def before_bwd(extra, needs, st):
         """Groups of several members: the gradient buffers exist before the lanes fork, so that members that share a
         parameter add to ONE buffer (the additions themselves are atomic)."""
-        for p, need in zip(saved[1:3], needs[1:3]):
+        for p, need in zip(extra[:2], needs[1:3]):
             if need:
                 LayerNorm._grad(p, st)
 
@@ -1900,13 +1904,13 @@ class GroupFn(torch.autograd.Function):
         needs_all = ctx.needs_input_grad[1:]
         spans, extras = ctx.spans, ctx.extras
         gouts = list(gouts)
-        for (op, _, _), (ipos, icnt, opos, ocnt, spos, scnt) in zip(members, spans):   # before the fork
+        for i, ((op, _, _), (ipos, icnt, opos, ocnt, _, _)) in enumerate(zip(members, spans)):   # before the fork
             own = getattr(op, 'LAYOUT', None)
             for k in range(opos, opos + ocnt):
                 if gouts[k] is not None and (own is not None or gouts[k].dim() == 4):
                     gouts[k] = (own or nhwc)(gouts[k])
             if nl > 1 and hasattr(op, 'before_bwd') and any(g is not None for g in gouts[opos:opos + ocnt]):
-                op.before_bwd(saved[spos:spos + scnt], needs_all[ipos:ipos + icnt], ctypes.c_void_p(cur.cuda_stream))
+                op.before_bwd(extras[i], needs_all[ipos:ipos + icnt], ctypes.c_void_p(cur.cuda_stream))
         _ensure_workspaces(dev, nl)
 
         def run_member(i, handle, lane):

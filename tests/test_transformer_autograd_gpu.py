@@ -14,6 +14,11 @@ def norm(form, x, gamma, beta):
     return o.layer_norm(x, gamma, beta) if form == 'single' else o.run_group([(o.LayerNorm, (x, gamma, beta), 1e-5)])[0]
 
 
+def check_all(x, gamma, beta, f):
+    assert all(t.grad is not None for t in (x, gamma, beta))
+    check_grads(x.grad, gamma.grad, beta.grad, f)
+
+
 def dense(t):
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -187,7 +192,7 @@ def test_forward_mode_through_the_backward_pass_is_refused():
             torch.autograd.grad(y, x, fwd_ad.make_dual(dy, torch.ones_like(dy)))
     assert gamma.grad is None
     y.backward(dy)
-    check_grads(x.grad, gamma.grad, beta.grad, formula(x, gamma, beta, dy, 1e-5))
+    check_all(x, gamma, beta, formula(x, gamma, beta, dy, 1e-5))
 
 
 @pytest.mark.parametrize('how', ['jit.trace', 'make_fx'])
@@ -204,7 +209,7 @@ def test_recording_is_refused(how):
             record(lambda g: torch.autograd.grad(y, x, g, retain_graph=True)[0], dy)
         assert gamma.grad is None
     y.backward(dy)
-    check_grads(x.grad, gamma.grad, beta.grad, formula(x, gamma, beta, dy, 1e-5))
+    check_all(x, gamma, beta, formula(x, gamma, beta, dy, 1e-5))
 
 
 def test_checkpointed_compiled_and_counted():
@@ -221,7 +226,7 @@ def test_checkpointed_compiled_and_counted():
         y = run(x)
         check_y(y, f)
         y.backward(dy)
-        check_grads(x.grad, gamma.grad, beta.grad, f)
+        check_all(x, gamma, beta, f)
     with FlopCounterMode(display=False), torch.no_grad():
         check_y(plain(x), f)
 
@@ -272,4 +277,22 @@ def test_what_is_no_plain_tensor_is_refused():
     with pytest.raises((RuntimeError, NotImplementedError)):
         torch.autograd.grad(y, x, torch.stack([dy, dy]), is_grads_batched=True, retain_graph=True)
     y.backward(dy)
-    check_grads(x.grad, gamma.grad, beta.grad, formula(x, gamma, beta, dy, 1e-5))
+    check_all(x, gamma, beta, formula(x, gamma, beta, dy, 1e-5))
+
+
+def test_parameters_behind_saved_tensor_hooks():
+    """The member's gamma and beta are not copies of the hooks': their gradients arrive, and a change of gamma is refused as ever."""
+    x, dy, gamma, beta = inputs((30, 72), torch.float32)
+    f = formula(x, gamma, beta, dy, 1e-5)
+    x.requires_grad_()
+    for form in ('single', 'group'):
+        x.grad = gamma.grad = beta.grad = None
+        with torch.autograd.graph.save_on_cpu():
+            y = norm(form, x, gamma, beta)
+        y.backward(dy)
+        check_all(x, gamma, beta, f)
+        y = norm(form, x, gamma, beta)
+        with torch.no_grad():
+            gamma.mul_(1.0)
+        with pytest.raises(RuntimeError):
+            y.backward(dy)
