@@ -1196,7 +1196,8 @@ def _row_stride(t):
 class LayerNorm:
     """y = (x - mean) / sqrt(var + eps) * gamma + beta over the channels: dim 1 of a 4-D NCHW map, the last dimension of
     tokens [..., C].  tensors = (x, gamma | None, beta | None); meta = eps.  x in fp32, bf16 or fp16 (y and its gradient have
-    x's type), gamma and beta fp32.  Rows may lie apart (a slice of wider tokens); other layouts are copied first."""
+    x's type), gamma and beta fp32.  Rows may lie apart (a slice of wider tokens); other layouts are copied first.  In a Chain:
+    fp32 maps, as a Chain's input and output slots are."""
     NHWC = (0,)
 
     @staticmethod
@@ -1570,6 +1571,8 @@ INBN = __import__('os').environ.get('ADVMIX_INBN', '1') != '0'        # BatchNor
 def _add(st, a, b):
     """a + b for two dense tensors of identical layout, on the member's stream (gradient fan-in
     inside a Chain; a torch add would run on the caller's stream)."""
+    if a.dtype != torch.float32 or b.dtype != torch.float32:
+        raise TypeError('advmix_amd: gradient fan-in of %s and %s, only fp32 tensors can have several readers in a Chain' % (a.dtype, b.dtype))
     if a.shape != b.shape or a.stride() != b.stride():
         raise RuntimeError('advmix_amd: gradient fan-in of differently laid out tensors')
     out = keep(torch.empty_like(a, memory_format=torch.preserve_format))

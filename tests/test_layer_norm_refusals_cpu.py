@@ -65,3 +65,10 @@ def test_what_only_watches_operations_is_not_refused():
     with FlopCounterMode(display=False), torch.device('cpu'):
         with pytest.raises(TypeError):
             ops.layer_norm(torch.randn(5, 8))
+
+
+def test_fan_in_of_16_bit_gradients():
+    """A Chain adds up the gradients of a tensor with several readers in fp32 only: anything else would be read past its end."""
+    for a, b in ((torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.bfloat16)):
+        with pytest.raises(TypeError, match='fan-in'):
+            ops._add(None, torch.zeros(2, 8, dtype=a), torch.zeros(2, 8, dtype=b))

@@ -296,3 +296,43 @@ def test_parameters_behind_saved_tensor_hooks():
             gamma.mul_(1.0)
         with pytest.raises(RuntimeError):
             y.backward(dy)
+
+
+def chain(o, subs, tensors, n_out):
+    return o.run_group([(o.Chain, tensors, (subs, (0,), n_out))])[0]
+
+
+def test_two_readers_of_one_map_in_a_chain():
+    """One map read by two layer norms of a chain: its gradient is the sum of theirs."""
+    o = ops()
+    x, dy, g1, b1 = inputs((2, 24, 6, 5), torch.float32)
+    _, dy2, _, _ = inputs((2, 24, 6, 5), torch.float32, seed=4)
+    g2, b2 = (torch.nn.Parameter(p.detach().flip(0).clone()) for p in (g1, b1))
+    subs = ((o.LayerNorm, (('s', 0), ('i', 1), ('i', 2)), 1e-5, 1), (o.LayerNorm, (('s', 0), ('i', 3), ('i', 4)), 1e-5, 2))
+    y1, y2 = chain(o, subs, (x.requires_grad_(), g1, b1, g2, b2), (1, 2))
+    torch.autograd.backward([y1, y2], [dy, dy2])
+    f1, f2 = formula(x, g1, b1, dy, 1e-5), formula(x, g2, b2, dy2, 1e-5)
+    check_y(y1, f1)
+    check_y(y2, f2)
+    check_grads(None, g1.grad, b1.grad, f1)
+    check_grads(None, g2.grad, b2.grad, f2)
+    n = 24 / 64 + 16                                        # both terms' own tolerances and a rounding of their sum
+    want, tol = f1['dx'] + f2['dx'], U * (f1['dx'] + f2['dx']).abs()
+    for f in (f1, f2):
+        top = f['h'].abs().amax(1, keepdim=True) * (1 + f['xh'].abs().amax(1, keepdim=True)) ** 2
+        tol = tol + (n * (f['R'] + 4) + 16) * U * f['rstd'] * top + U * f['dx'].abs()
+    check('dx', x.grad.permute(0, 2, 3, 1).reshape(-1, 24), want, tol)
+
+
+def test_two_readers_of_a_16_bit_tensor_in_a_chain_are_refused():
+    """Refused on the host when the second gradient would be added."""
+    o = ops()
+    x, dy, g, b = inputs((2, 24, 6, 5), torch.float32)
+    t = inputs((40, 24), torch.bfloat16)[0].requires_grad_()
+    subs = ((o.LayerNorm, (('i', 1), ('i', 2), ('i', 3)), 1e-5, 1), (o.LayerNorm, (('i', 1), ('i', 2), ('i', 3)), 1e-5, 2))
+    y1, y2 = chain(o, subs, (x, t, g, b), (1, 2))
+    with pytest.raises(TypeError, match='fan-in'):
+        torch.autograd.backward([y1, y2], [torch.ones_like(y1), torch.ones_like(y2)])
+    for bad in (x.bfloat16(), x.reshape(48, 30)):
+        with pytest.raises((TypeError, ValueError)):        # what a chain's slots are
+            chain(o, ((o.LayerNorm, (('s', 0), None, None), 1e-5, 1),), (bad,), (1,))
