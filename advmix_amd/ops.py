@@ -1301,7 +1301,7 @@ class LayerNorm:
         return g
 
     @staticmethod
-    def before_bwd(extra, needs, st):
+    def before_bwd(extra, meta, needs, st):
         """Groups of several members: the gradient buffers exist before the lanes fork, so that members that share a
         parameter add to ONE buffer (the additions themselves are atomic)."""
         for p, need in zip(extra[:2], needs[1:3]):
@@ -1705,6 +1705,13 @@ class Chain:
         return plan
 
     @staticmethod
+    def before_bwd(rec, meta, needs, st):
+        """Its layer norms' (chains of one group run on different lanes and may share parameters)."""
+        for (op, _r, smeta, _d), (_sp, _sc, ex, nin) in zip(meta[0], rec):
+            if op is LayerNorm:
+                op.before_bwd(ex, smeta, nin, st)
+
+    @staticmethod
     def bwd(st, lane, saved, rec, meta, grads, needs):
         subs, ext_slots, out_slots = meta[:3]
         plan = (meta[3] if len(meta) > 3 else Chain.bnb_plan(subs)) if BNB_FUSED else {}
@@ -1913,7 +1920,7 @@ class GroupFn(torch.autograd.Function):
                 if gouts[k] is not None and (own is not None or gouts[k].dim() == 4):
                     gouts[k] = (own or nhwc)(gouts[k])
             if nl > 1 and hasattr(op, 'before_bwd') and any(g is not None for g in gouts[opos:opos + ocnt]):
-                op.before_bwd(extras[i], needs_all[ipos:ipos + icnt], ctypes.c_void_p(cur.cuda_stream))
+                op.before_bwd(extras[i], members[i][2], needs_all[ipos:ipos + icnt], ctypes.c_void_p(cur.cuda_stream))
         _ensure_workspaces(dev, nl)
 
         def run_member(i, handle, lane):

@@ -336,3 +336,22 @@ def test_two_readers_of_a_16_bit_tensor_in_a_chain_are_refused():
     for bad in (x.bfloat16(), x.reshape(48, 30)):
         with pytest.raises((TypeError, ValueError)):        # what a chain's slots are
             chain(o, ((o.LayerNorm, (('s', 0), None, None), 1e-5, 1),), (bad,), (1,))
+
+
+def test_chains_of_one_group_that_share_parameters():
+    """Two chains, two lanes, the second one's input far longer on its way: one gradient for gamma and beta, both parts in it."""
+    o = ops()
+    sets = [inputs((2, 24, 6, 5), torch.float32), inputs((4, 24, 48, 40), torch.float32, seed=3)]
+    gamma, beta = sets[0][2:]
+    for _ in range(3):
+        gamma.grad = beta.grad = None
+        sub = ((o.LayerNorm, (('s', 0), ('i', 1), ('i', 2)), 1e-5, 1),)
+        ys = o.run_group([(o.Chain, (x.requires_grad_(), gamma, beta), (sub, (0,), (1,))) for x, _, _, _ in sets])
+        for x, _, _, _ in sets:
+            x.grad = None
+        torch.autograd.backward([y for (y,) in ys], [dy for _, dy, _, _ in sets])
+        fs = [formula(x, gamma, beta, dy, 1e-5) for x, dy, _, _ in sets]
+        for (x, _, _, _), f in zip(sets, fs):
+            check_grads(x.grad, None, None, f)
+        check_sum(gamma.grad, fs, 'dg')
+        check_sum(beta.grad, fs, 'db')
