@@ -290,14 +290,14 @@ class FlatAdamW(FlatAdam):
             raise ValueError('FlatAdamW: no elements to train')
         self._hyper_tuple()
 
-    def _hyper_tuple(self):
-        """One row of doubles per group behind one for the whole step, checked."""
+    def _hyper_tuple(self, groups=None):
+        """One row of doubles per group (of the optimizer's own if none are given) behind one for the whole step, checked."""
         if (self.max_norm is not None) != self._clips:
             raise ValueError('FlatAdamW: whether the step clips is decided by the constructor')
         if self._clips and not 0 < float(self.max_norm) < float('inf'):
             raise ValueError('FlatAdamW: max_norm must be positive and finite, got %r' % (self.max_norm,))
         rows = [float(self.max_norm) if self._clips else 0.0] + [0.0] * (self.HYPER - 1)
-        for g in self.param_groups:
+        for g in self.param_groups if groups is None else groups:
             lr, (b1, b2), eps, wd = float(g['lr']), g['betas'], float(g['eps']), float(g['weight_decay'])
             if g.get('amsgrad') or g.get('maximize'):
                 raise ValueError('FlatAdamW: amsgrad and maximize are not supported')
@@ -425,8 +425,11 @@ class FlatAdamW(FlatAdam):
         sizes = [len(g['params']) for g in sd['param_groups']]
         if sizes != [len(g['params']) for g in self.param_groups]:
             raise ValueError('FlatAdamW: the state has other parameter groups (%r parameters)' % (sizes,))
+        # check everything before anything is overwritten
+        merged = [dict(g, **{k: v for k, v in new.items() if k != 'params'}) for g, new in zip(self.param_groups, sd['param_groups'])]
+        self._hyper_tuple(merged)
         todo, fresh = [], []
-        for i, p in enumerate(ps):                            # check everything before anything is overwritten
+        for i, p in enumerate(ps):
             st = sd['state'].get(i) or sd['state'].get(str(i))
             if st is None:
                 fresh.append((i, p))
@@ -436,21 +439,15 @@ class FlatAdamW(FlatAdam):
                 if full in st:
                     if st[full].shape != p.shape:
                         raise ValueError('FlatAdamW: %s of parameter %d has another shape' % (full, i))
-                elif codes not in st or scale not in st or st[codes].shape != p.shape or st[scale].numel() != hi - lo \
+                elif codes not in st or scale not in st or st[codes].shape != p.shape or st[scale].shape != (hi - lo,) \
                         or st[codes].dtype not in (torch.float8_e4m3fn, torch.uint8) \
                         or st[scale].dtype not in (torch.float8_e8m0fnu, torch.uint8):
                     raise ValueError('FlatAdamW: the state of parameter %d lacks %s, or its codes have another shape or type' % (i, full))
-            float(st['step'])
+            if not 0 <= float(st['step']) < 2 ** 53:
+                raise ValueError('FlatAdamW: the state of parameter %d has a step of %r' % (i, st['step']))
             todo.append((i, p, st))
-        before = [dict(g) for g in self.param_groups]
-        for g, new in zip(self.param_groups, sd['param_groups']):
-            g.update({k: v for k, v in new.items() if k != 'params'})
-        try:
-            self._hyper_tuple()
-        except ValueError:
-            for g, old in zip(self.param_groups, before):
-                g.update(old)
-            raise
+        for g, new in zip(self.param_groups, merged):
+            g.update(new)
         step = 0
         byte = lambda t: t.view(torch.uint8) if t.element_size() == 1 else t          # noqa: E731
         P = lambda t, at=0: ctypes.c_void_p(t.data_ptr() + at)          # noqa: E731
