@@ -99,11 +99,15 @@ def build(force=False, verbose=True):
             if verbose:
                 print(' '.join(cmd), flush=True)
             procs.append((s, obj, subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True)))
+    node_error = None                                       # (told when the library is there: only one op needs the module)
     if force or _stale_object(NODE, NODE_SO, os.path.join(CSRC, NODE), [], info):
         cmd = _node_command()
         if verbose:
             print(' '.join(cmd), flush=True)
-        procs.append((NODE, NODE_SO, subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True)))
+        try:
+            procs.append((NODE, NODE_SO, subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True)))
+        except OSError as e:
+            node_error = str(e)
     bad = []
     for s, obj, p in procs:
         _, err = p.communicate()
@@ -114,7 +118,9 @@ def build(force=False, verbose=True):
             print('\n'.join(msgs), flush=True)
         if p.returncode != 0:
             sys.stderr.write(err[-4000:])
-            raise RuntimeError(('the C++ compiler' if s == NODE else 'hipcc') + ' failed on ' + s)
+            if s != NODE:
+                raise RuntimeError('hipcc failed on ' + s)
+            node_error = 'the C++ compiler failed'
         users = _scratch_users(err)
         if users:
             os.remove(obj)                                  # never link it
@@ -129,7 +135,9 @@ def build(force=False, verbose=True):
             print(' '.join(cmd), flush=True)
         subprocess.check_call(cmd)
         linked = True
-    _record(hipcc, [s for s, _, _ in procs], linked)
+    _record(hipcc, [s for s, _, _ in procs if s != NODE or node_error is None], linked)
+    if node_error is not None:
+        raise RuntimeError('%s on %s (the library itself is built)' % (node_error, NODE))
     return SO
 
 

@@ -354,4 +354,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_node", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__node(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__node(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", ADVMIX_TORCH) != 0) Py_CLEAR(m);      // (torch's C++ types are not the same from one to the next)
+    return m;
+}

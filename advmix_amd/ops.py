@@ -23,12 +23,15 @@ import torch
 
 from ._lib import call, lib
 
-try:                                                       # the layer norm's autograd node (csrc/layer_norm_node.cpp): host code only,
-    from . import _node                                    # it calls the library's entry points by address
+try:                                                       # the node of a layer norm by itself (csrc/layer_norm_node.cpp): host code only,
+    from . import _node                                    # it calls the library's entry points by address.  Nothing else here needs it, or
+    if _node.torch_version != torch.__version__:           # knows torch's types: without it that one op raises
+        raise ImportError('built for torch %s, this is %s' % (_node.torch_version, torch.__version__))
+    _node.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.advmix_layer_norm_fwd, lib.advmix_layer_norm_bwd,
+                                                                 lib.advmix_layer_norm_parts)))
+    _node_error = None
 except ImportError as e:
-    raise ImportError('advmix_amd: _node.so not found or not for this torch (%s) - build it with `python -m advmix_amd.build`' % e)
-_node.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.advmix_layer_norm_fwd, lib.advmix_layer_norm_bwd,
-                                                             lib.advmix_layer_norm_parts)))
+    _node, _node_error = None, str(e)
 
 ACT_NONE, ACT_RELU, ACT_LEAKY = 0, 1, 2
 _CL = torch.channels_last
@@ -1295,7 +1298,8 @@ class LayerNorm:
     def _grad(p, st):
         fresh = p.grad is None and getattr(p, '_flat_grad_view', None) is None
         g = _grad_buf(p, st)
-        (_node.first_written_here if fresh else _node.wait_for_first_write)(g)      # (a layer norm by itself may run on another stream)
+        if _node is not None:                              # (a layer norm by itself may run on another stream)
+            (_node.first_written_here if fresh else _node.wait_for_first_write)(g)
         if g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape or g.device != p.device:
             raise RuntimeError('layer_norm: a parameter\'s .grad must be a contiguous fp32 tensor of its shape')
         return g
@@ -1999,6 +2003,9 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5):
     parameters' gradients are summed in fp32 in a fixed order; those gradients are accumulated into ``.grad`` as everywhere
     here.  No second derivative.  A backward pass may be captured into a HIP graph while an eager graph of the same gamma and
     beta is alive; with torch, not while one of the same leaf x is."""
+    if _node is None:
+        raise ImportError('advmix_amd: _node.so is not there or not for this torch (%s) - build it with `python -m advmix_amd.build`; '
+                          'ops.LayerNorm in a launch group (run_group) does without' % _node_error)
     return _node.layer_norm(x, gamma, beta, eps, getattr(gamma, '_flat_grad_view', None), getattr(beta, '_flat_grad_view', None))
 
 
