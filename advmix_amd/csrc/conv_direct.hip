@@ -822,7 +822,7 @@ int launch(ConvD& p, int64_t Mmax, hipStream_t st, int64_t stats_cap) {
         case CFG_64x64_GRID_SPLIT:                                         // K across gridDim.z + atomics
             if (p.bn_gamma || (MODE == 0 && p.res) || p.act || p.stats || p.bnb_c) return -2;   // fused epilogue needs whole-K tiles
             p.nsplit = ns;
-            if (hipMemsetAsync(p.y, 0, (size_t)p.N * p.Ho * p.Wo * p.Co * sizeof(float), st) != hipSuccess)
+            if (advmix_fill(p.y, 0.f, (int64_t)p.N * p.Ho * p.Wo * p.Co, st) != ADVMIX_OK)      // (a kernel: no memset node in a caller's graph)
                 return ADVMIX_ELAUNCH;
             LAUNCHD(1, 1, 2, 2, true);
             break;

@@ -514,7 +514,7 @@ extern "C" int advmix_conv4x4s2_wino_wgrad(const float* hi, const float* lo, flo
     hipLaunchKernelGGL(w4::wino4_output_adj, dim3(cdiv((int64_t)p.rows * (Cl / 4), 256)), dim3(256), 0, st, lo, dm, N, H / 2, W / 2, Cl,
                        p.Th, p.Tw, p.tiles, p.rows);
     ADVMIX_CHECK_LAUNCH();
-    if (hipMemsetAsync(du, 0, (size_t)16 * Cl * K * sizeof(float), st) != hipSuccess) return ADVMIX_ELAUNCH;
+    if (advmix_fill(du, 0.f, (int64_t)16 * Cl * K, st) != ADVMIX_OK) return ADVMIX_ELAUNCH;      // (a kernel: no memset node in a caller's graph)
     const float* a[16];
     const float* b[16];
     float* d[16];
