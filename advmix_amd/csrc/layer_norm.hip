@@ -514,10 +514,11 @@ int parts_of(int64_t rows, int C, int V) {
     return (int)((units + each - 1) / each);
 }
 
-#define HOLDS(CASE)                                                                                          \
-    CASE(1, 1) CASE(2, 1) CASE(4, 1) CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2) CASE(256, 1) \
-    CASE(256, 2) CASE(1024, 1) CASE(1024, 2)
+// what hold_of returns: for every type, for fp32, for 16 bits
+#define HOLDS(CASE)                                                                                               \
+    CASE(1, 1) CASE(2, 1) CASE(4, 1) CASE(8, 1) CASE(16, 1) CASE(32, 1) CASE(64, 1) CASE(64, 2) CASE(256, 2) CASE(1024, 2)
 #define HOLDS_F32(CASE) CASE(64, 3) CASE(64, 4) CASE(256, 3) CASE(256, 4) CASE(1024, 4)
+#define HOLDS_16(CASE) CASE(256, 1) CASE(1024, 1)
 
 template <typename T>
 int fwd(const void* x_, int64_t ldx, const float* gamma, const float* beta, void* y_, float* mean, float* rstd, int64_t rows, int C,
@@ -533,13 +534,14 @@ int fwd(const void* x_, int64_t ldx, const float* gamma, const float* beta, void
     const dim3 g((unsigned)grid);
 #define FWD(L_, NV_)                                                                                                            \
     if (h.L == L_ && h.NV == NV_) {                                                                                             \
-        if (C % V) hipLaunchKernelGGL((ln_fwd_kernel<T, L_, NV_, true>), g, dim3(threads_of(L_)), 0, st, x, ldx, gamma, beta, y, \
-                                      mean, rstd, rows, C, eps);                                                                \
+        constexpr bool ODD = L_ > 1;                             /* (one lane holds one whole chunk or nothing) */              \
+        if (ODD && C % V) hipLaunchKernelGGL((ln_fwd_kernel<T, L_, NV_, ODD>), g, dim3(threads_of(L_)), 0, st, x, ldx, gamma,   \
+                                             beta, y, mean, rstd, rows, C, eps);                                                \
         else hipLaunchKernelGGL((ln_fwd_kernel<T, L_, NV_, false>), g, dim3(threads_of(L_)), 0, st, x, ldx, gamma, beta, y, mean, \
                                 rstd, rows, C, eps);                                                                            \
     }
     HOLDS(FWD)
-    if constexpr (V == 4) { HOLDS_F32(FWD) }
+    if constexpr (V == 4) { HOLDS_F32(FWD) } else { HOLDS_16(FWD) }
 #undef FWD
     if (h.L == 0) {
         if (C < V) hipLaunchKernelGGL((ln_fwd_walk_kernel<T, 64>), dim3((unsigned)(rows < 8192 ? rows : 8192)), dim3(64), 0, st, x, ldx, gamma, beta, y, mean, rstd, rows, C, eps);
@@ -570,15 +572,16 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         const bool past = rows * C * (int64_t)sizeof(T) * 3 > (256ll << 20);
 #define BWD(L_, NV_)                                                                                                             \
     if (h.L == L_ && h.NV == NV_) {                                                                                              \
-        if (C % V) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, true, false>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, gamma, \
-                                      mean, rstd, dx, dgamma, dbeta, pp, add, rows, C);                                          \
+        constexpr bool ODD = L_ > 1;                                                                                             \
+        if (ODD && C % V) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, ODD, false>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, \
+                                             gamma, mean, rstd, dx, dgamma, dbeta, pp, add, rows, C);                            \
         else if (past) hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, false, true>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, \
                                           ldx, gamma, mean, rstd, dx, dgamma, dbeta, pp, add, rows, C);                          \
         else hipLaunchKernelGGL((ln_bwd_kernel<T, L_, NV_, false, false>), g, dim3(TH), lds > box ? lds : box, st, dy, lddy, x, ldx, \
                                 gamma, mean, rstd, dx, dgamma, dbeta, pp, add, rows, C);                                         \
     }
         HOLDS(BWD)
-        if constexpr (V == 4) { HOLDS_F32(BWD) }
+        if constexpr (V == 4) { HOLDS_F32(BWD) } else { HOLDS_16(BWD) }
 #undef BWD
         if (!sums || !pp) { ADVMIX_CHECK_LAUNCH(); return ADVMIX_OK; }
     } else {
