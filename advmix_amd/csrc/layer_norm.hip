@@ -445,6 +445,11 @@ __global__ __launch_bounds__(TH) void ln_fwd_walk_kernel(const T* __restrict__ x
     }
 }
 
+// A product rounded by itself: the same number where it is summed and where the mean is taken off it, so that one channel's dx is 0.
+__device__ __forceinline__ float rounded(float a, float b) {
+#pragma clang fp contract(off)
+    return a * b;
+}
 template <typename T, int TH>
 __global__ __launch_bounds__(TH) void ln_dx_walk_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
                                                         const float* __restrict__ gamma, const float* __restrict__ mean,
@@ -456,14 +461,14 @@ __global__ __launch_bounds__(TH) void ln_dx_walk_kernel(const T* __restrict__ dy
         const float mu = mean[r], is = rstd[r];
         float a = 0.f, b = 0.f;
         for (int c = threadIdx.x; c < C; c += TH) {
-            const float h = Vec<T>::ld(gr + c) * (gamma ? gamma[c] : 1.f);
+            const float h = rounded(Vec<T>::ld(gr + c), gamma ? gamma[c] : 1.f);
             a += h;
             b += h * ((Vec<T>::ld(xr + c) - mu) * is);
         }
         a = row_sum<TH, TH>(a, box, flip) / C;
         b = row_sum<TH, TH>(b, box, flip) / C;
         for (int c = threadIdx.x; c < C; c += TH) {
-            const float h = Vec<T>::ld(gr + c) * (gamma ? gamma[c] : 1.f);
+            const float h = rounded(Vec<T>::ld(gr + c), gamma ? gamma[c] : 1.f);
             Vec<T>::st(dx + r * C + c, is * (h - a - (Vec<T>::ld(xr + c) - mu) * is * b));
         }
     }

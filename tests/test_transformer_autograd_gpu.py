@@ -355,3 +355,16 @@ def test_chains_of_one_group_that_share_parameters():
             check_grads(x.grad, None, None, f)
         check_sum(gamma.grad, fs, 'dg')
         check_sum(beta.grad, fs, 'db')
+
+
+@pytest.mark.parametrize('kind', [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize('shape', [(1, 1), (4096, 1), (3, 1, 8, 6)], ids=str)
+def test_one_channel(shape, kind):
+    """The norm of one number is 0 whatever it is: y is beta, and x and gamma have a gradient of 0, to the bit."""
+    x, dy, gamma, beta = inputs(shape, kind)
+    y = ops().layer_norm(x.requires_grad_(), gamma, beta)
+    y.backward(dy)
+    assert torch.equal(y, beta.detach().to(kind).expand_as(y))
+    assert not x.grad.any() and not gamma.grad.any()
+    f = formula(x, gamma, beta, dy, 1e-5)
+    check_grads(None, None, beta.grad, f)
