@@ -209,8 +209,9 @@ template <bool NT, typename T> __device__ __forceinline__ void stv(T* p, T v) {
 __device__ __forceinline__ const f32x4* quad(const float* p) { return reinterpret_cast<const f32x4*>(p); }
 __device__ __forceinline__ f32x4* quad(float* p) { return reinterpret_cast<f32x4*>(p); }
 
-// Bound by memory: 28 bytes an element, 28.5 M elements 138 us = 5.8 TB/s.  A workgroup takes one chunk and ends (walking workgroups
-// with the next chunk on its way are slower: through the caches 170 us with 2048 of them, 155 us this way).
+// Bound by memory: 28 bytes an element, 28.5 M elements in 300 tensors 138 us = 5.8 TB/s (in 30 tensors 131 us).  A workgroup takes one
+// chunk and ends (walking workgroups with the next chunk on its way are slower: through the caches 170 us with 2048 of them, 151 us
+// this way).
 template <bool NT, bool OWN>
 __global__ __launch_bounds__(256) void adamw_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ m,
                                                     float* __restrict__ v, const Row* __restrict__ table, Step step) {
@@ -311,8 +312,9 @@ __device__ __forceinline__ int block_exponent(const float (&x)[4], bool in, bool
     return exponent_byte(t);
 }
 
-// 16 bytes an element and some 90 instructions, 28.5 M elements 85 us = 5.4 TB/s: close to where the vector units would bound it, hence the conversion instructions,
-// the roots off one instruction and maxima without LDS (146 instructions an element and 103 us for 28.5 M elements without them).
+// 16 bytes an element and some 90 instructions, 28.5 M elements in 300 tensors 82 us = 5.5 TB/s: close to where the vector units would
+// bound it, hence the conversion instructions, the roots off one instruction and maxima without LDS (146 instructions an element and
+// 103 us without them).
 template <bool NT, bool OWN>
 __global__ __launch_bounds__(256) void adamw8_kernel(float* __restrict__ p, const float* __restrict__ g, uint8_t* __restrict__ m,
                                                      uint8_t* __restrict__ r, uint8_t* __restrict__ ms, uint8_t* __restrict__ rs,
@@ -401,14 +403,14 @@ __global__ __launch_bounds__(256) void unpack8_kernel(const uint8_t* __restrict_
     }
 }
 
-// What a step touches, from its chunks, against the last-level cache of 256 MB.  Past the caches / through them, us: 63.6 M elements
-// in 32 bits (1.8 GB, clipped) 320 / 396, 28.5 M (800 MB) 138 / 152, 10 M (280 MB) 50 / 57, 3 M (84 MB) 18.8 / 17.4; in 8 bits 28.5 M
-// (456 MB) 85.6 / 89.2, 10 M (160 MB) 33.6 / 33.2.
+// What a step touches, from its chunks, against the last-level cache of 256 MB.  Past the caches / through them, us (steps replayed
+// from a HIP graph, three optimizers in turn): 63.6 M elements in 32 bits (1.8 GB, clipped) 306 / 392, 28.5 M (800 MB) 131 / 151, 10 M
+// (280 MB) 50 / 57, 3 M (84 MB) 17.6 / 16.4; in 8 bits 28.5 M (456 MB) 79 / 86, 10 M (160 MB) 31.6 / 32.0, 3 M (48 MB) 12.9 / 12.8.
 bool stream_past(int chunks, int bytes) { return (int64_t)chunks * 1024 * bytes > (256ll << 20); }
 
 // In a small step each workgroup works out the coefficients for itself (two powers by squaring, hidden behind its loads): a launch
-// less.  Itself / a launch before, us in 32 bits: 20 000 elements 3.8 / 5.0, 100 000 4.6 / 5.1, 200 000 5.7 / 5.5 (the tickets queue
-// up), and 4 us of host time in each.
+// less.  Itself / a launch before, us: 20 000 elements 3.4 / 4.5 in 32 bits and 4.0 / 5.1 in 8, 100 000 4.4 / 4.7 and 4.9 / 5.2, 200 000
+// 5.4 / 4.9 and 6.0 / 5.3, 1 000 000 16.8 / 8.5 and 15.9 / 7.3 (the tickets queue up), and 4 us of host time in each.
 bool on_its_own(int chunks) { return chunks <= 128; }
 
 bool step_ok(const void* p, const void* g, const void* table, int chunks, const Step& s) {

@@ -166,9 +166,10 @@ template <int V> __device__ __forceinline__ void params(float (&to)[V], const fl
 
 constexpr int threads_of(int L) { return L > 256 ? L : 256; }
 
-// One reading, one writing: 12289 x 2048 fp32 33.5 us = 6.0 TB/s, 16384 x 4096 bf16 46 us = 5.8 TB/s, 32 x 64 x 48 pixels of 32
-// channels 6.1 us.  Workgroups walk the rows, so that gamma and beta are read once; without the next row on its way the second case
-// takes 66 us.
+// (Times here and below: launches replayed from a HIP graph, three sets of data in turn, each with outputs of its own.)
+// One reading, one writing: 12289 x 2048 fp32 38 us = 5.2 TB/s (33 us = 6.1 TB/s where y is the memory of the call before), 16384 x
+// 4096 bf16 53 us = 5.1 TB/s (46 us), 32 x 64 x 48 pixels of 32 channels 6.1 us.  Workgroups walk the rows, so that gamma and beta
+// are read once; without the next row on its way the second case's 46 us are 66.
 template <typename T, int L, int NV, bool TAIL>
 __global__ __launch_bounds__(threads_of(L)) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
                                                                const float* __restrict__ beta, T* __restrict__ y,
@@ -245,8 +246,8 @@ __device__ __forceinline__ void give(float* to, int64_t c, float v, int add) {
 
 // part[workgroup][0][c] = sum of dy * xh, [1][c] = sum of dy over the workgroup's rows; a launch of one workgroup gives its sums
 // to dgamma and dbeta itself (part NULL; not one of long rows, whose lanes would write them one element at a time).
-// Two readings, one writing: 16384 x 4096 bf16 69 us = 5.9 TB/s, 100000 x 256 fp32 52 us = 5.9 TB/s, the same without the sums 69 and
-// 50 us.  Vector work matters: with masks per element instead of per chunk the first case takes 77 us.
+// Two readings, one writing, with the folding launch: 16384 x 4096 bf16 76 us = 5.3 TB/s, 100000 x 256 fp32 58 us = 5.3 TB/s, the same
+// without the sums 73 and 57 us.  Vector work matters: masks per element instead of per chunk are 8 us more in the first case.
 // PAST: x is read past the caches (dy is what another kernel has just left there).
 template <typename T, int L, int NV, bool TAIL, bool PAST>
 __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
@@ -396,7 +397,7 @@ __global__ __launch_bounds__(L > 512 ? L : 512) void ln_bwd_kernel(const T* __re
 }
 
 // The workgroups' partial sums in a fixed order: 16 columns x 64 slices of the partial rows per workgroup, so that a thread has at
-// most eight loads, all in flight (2.8 - 3 us, a launch's own time; 4.3 us for 4096 columns).  With ``add`` ONE atomic addition per
+// most eight loads, all in flight (2.5 - 3.8 us, a launch's own time; 5 us for 4096 columns).  With ``add`` ONE atomic addition per
 // sum, so that two launches that add to one gradient (or one launch whose dgamma and dbeta are one) lose neither's part; a launch
 // that stores is for a gradient that no other one touches before it has run.
 constexpr int FOLD = 16;
@@ -423,6 +424,8 @@ __global__ __launch_bounds__(1024) void ln_fold_kernel(const float* __restrict__
 }
 
 // ---- rows that no workgroup holds (or fewer channels than a chunk): a workgroup walks the row, element by element -------
+// Built to be right, not fast: below a chunk at most seven lanes of a wave have an element and the column kernel as many of its 256
+// threads (70001 x 3 fp32 17 us forward and 48 backward, 100000 x 7 bf16 25 and 85, where memory would take 1).
 template <typename T, int TH>
 __global__ __launch_bounds__(TH) void ln_fwd_walk_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ gamma,
                                                          const float* __restrict__ beta, T* __restrict__ y, float* __restrict__ mean,
@@ -514,7 +517,7 @@ int parts_of(int64_t rows, int C, int V) {
     if (h.L == 0) return (int)(rows < 256 ? rows : 256);         // column kernel: slices of the rows
     const int R = (h.L > 512 ? h.L : 512) / h.L;
     const int64_t units = (rows + R - 1) / R, most = h.L == 1024 || h.NV * V >= 16 ? 256 : 512;
-    if (R > 1 && units <= 2) return 1;                           // (one workgroup, no folding: 16 x 768 bf16 5.3 us, 6.3 with two)
+    if (R > 1 && units <= 2) return 1;                           // (one workgroup, no folding: 16 x 768 bf16 5.1 us, 1 us more with two)
     const int64_t each = (units + most - 1) / most;
     return (int)((units + each - 1) / each);
 }
@@ -571,9 +574,10 @@ int bwd(const void* dy_, int64_t lddy, const void* x_, int64_t ldx, const float*
         const dim3 g((unsigned)(sums ? parts : (need < 2048 ? need : 2048)));
         const size_t lds = sums && R > 1 ? sizeof(float) * ((R < W ? R : W) * (size_t)(C % V ? C + (C >> 3) + 1 : C)) : 0, box = sizeof(float) * 2 * W;
         float* pp = parts > 1 || R == 1 ? part : nullptr;
-        // x, dy and dx against the last-level cache of 256 MB.  x read past the caches / through them, us: 30000 x 1024 fp32 (369 MB)
-        // 61 / 71, 100000 x 256 fp32 (307 MB) 52 / 56, 16384 x 4096 bf16 (403 MB) 78 / 79; 6144 x 768 bf16 (28 MB) 11.8 / 11.4.  With
-        // dy past them too the pass behind a forward pass loses 6 - 12 %.  (Odd widths keep to the caches: neighbouring rows share lines.)
+        // x, dy and dx against the last-level cache of 256 MB.  x read past the caches / through them, us, alone and with the forward
+        // pass before it: 30000 x 1024 fp32 (369 MB) 69 / 72 and 109 / 112, 16384 x 4096 bf16 (403 MB) 76 / 79 and 125 / 129, 100000 x
+        // 256 fp32 (307 MB) 58 / 61 and 96 / 93; 6144 x 768 bf16 (28 MB) 11.3 / 10.8 and 17.1 / 16.5.  With dy past them too the pass
+        // behind a forward pass loses 6 - 12 %.  (Odd widths keep to the caches: neighbouring rows share lines.)
         const bool past = rows * C * (int64_t)sizeof(T) * 3 > (256ll << 20);
 #define BWD(L_, NV_)                                                                                                             \
     if (h.L == L_ && h.NV == NV_) {                                                                                              \
