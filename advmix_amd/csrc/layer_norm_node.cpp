@@ -117,7 +117,9 @@ struct Capture {
     unsigned long long id = 0;
     explicit Capture(hipStream_t s) {
         hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (s != nullptr && hipStreamGetCaptureInfo(s, &status, &id) == hipSuccess) active = status == hipStreamCaptureStatusActive;
+        if (s == nullptr) return;
+        if (hipStreamGetCaptureInfo(s, &status, &id) == hipSuccess) active = status == hipStreamCaptureStatusActive;
+        else (void)hipGetLastError();                            // (not the next launch's)
     }
 };
 void wait_for_first_write(const at::Tensor& grad) {

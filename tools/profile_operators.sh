@@ -1,5 +1,5 @@
 #!/bin/bash
-# Times and counters of the layer norm and AdamW (run on the GPU box from the repo root): profile_operators.sh <folder under gpurun_out>
+# Times and counters of the layer norm and AdamW (from the repository root, on a machine with the GPU): profile_operators.sh <folder under gpurun_out>
 # Each counter in a run of its own, kernel trace only.
 R=$PWD; OUT=$R/gpurun_out/$1; mkdir -p $OUT
 timeout -k 10 120 python3 tools/bench_operators.py > $OUT/cases.log 2>&1 || exit 1
