@@ -31,7 +31,7 @@ def _node_command():
     return [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
             '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch.compiled_with_cxx11_abi(), '-I' + inc, '-I' + os.path.join(inc, 'torch/csrc/api/include'),
             '-I' + os.path.join(rocm, 'include'), '-I' + sysconfig.get_paths()['include'], os.path.join(CSRC, NODE), '-o', NODE_SO,
-            '-L' + lib, '-ltorch_python', '-ltorch_cpu', '-ltorch', '-lc10', '-lc10_hip', '-lamdhip64', '-DADVMIX_TORCH="%s"' % torch.__version__]
+            '-L' + lib, '-L' + os.path.join(rocm, 'lib'), '-ltorch_python', '-ltorch_cpu', '-ltorch', '-lc10', '-lc10_hip', '-lamdhip64', '-DADVMIX_TORCH="%s"' % torch.__version__]
 
 
 def _scratch_users(report):

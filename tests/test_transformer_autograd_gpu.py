@@ -368,3 +368,24 @@ def test_one_channel(shape, kind):
     assert not x.grad.any() and not gamma.grad.any()
     f = formula(x, gamma, beta, dy, 1e-5)
     check_grads(None, None, beta.grad, f)
+
+
+def test_gradients_are_ordinary_tensors(tmp_path):
+    """Gradients that a pass has made carry a note of their stream: they save, copy and step like any other."""
+    import copy
+    x, dy, gamma, beta = inputs((30, 72), torch.float32)
+    ops().layer_norm(x, gamma, beta).backward(dy)
+    f = formula(x, gamma, beta, dy, 1e-5)
+    torch.save([gamma.grad, beta.grad], str(tmp_path / 'g.pth'))
+    for dg, db in ([gamma.grad, beta.grad], torch.load(str(tmp_path / 'g.pth'), weights_only=True), copy.deepcopy([gamma.grad, beta.grad]),
+                   [t.clone() for t in (gamma.grad, beta.grad)], [t.detach() for t in (gamma.grad, beta.grad)],
+                   [torch.compile(lambda t: t * 1, backend='eager')(t) for t in (gamma.grad, beta.grad)]):
+        check_grads(None, dg, db, f)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in (gamma, beta)]
+    for p, q in zip((gamma, beta), twin):
+        q.grad = p.grad.clone()
+    norms = [torch.nn.utils.clip_grad_norm_(ps, 0.5) for ps in ((gamma, beta), twin)]
+    assert torch.equal(*norms)
+    for ps in ((gamma, beta), twin):
+        torch.optim.AdamW(ps, foreach=True).step()
+    assert all(torch.equal(p, q) and torch.equal(p.grad, q.grad) for p, q in zip((gamma, beta), twin))
