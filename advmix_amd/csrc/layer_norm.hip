@@ -632,6 +632,7 @@ extern "C" int advmix_layer_norm_bwd(const void* dy, int64_t lddy, const void* x
                                      int dtype, void* stream) {
     if (!dy || !x || !mean || !rstd || ldx < 0 || lddy < 0 || !sizes_ok(rows, C, dtype)) return ADVMIX_EINVAL;
     if ((dgamma || dbeta) && !part) return ADVMIX_EINVAL;
+    if (dgamma && dgamma == dbeta && (add & 3) != 3) return ADVMIX_EINVAL;       // (two sums in one place can only be added)
     if (!dx && !dgamma && !dbeta) return ADVMIX_OK;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == ADVMIX_F32) return bwd<float>(dy, lddy, x, ldx, gamma, mean, rstd, dx, dgamma, dbeta, part, add, rows, C, st);

@@ -2001,7 +2001,8 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-5):
     """Layer norm over dim 1 of a 4-D NCHW map (channels_last memory: every pixel by itself) or over the last dimension of
     tokens [..., C] (1-D to 3-D).  x: fp32, bf16 or fp16; gamma, beta: fp32 [C] parameters or None.  The statistics and the
     parameters' gradients are summed in fp32 in a fixed order; those gradients are accumulated into ``.grad`` as everywhere
-    here.  No second derivative.  A backward pass may be captured into a HIP graph while an eager graph of the same gamma and
+    here.  No second derivative, no forward mode, and nothing that records or transforms operations (jit.trace, make_fx,
+    torch.func): those raise.  A backward pass may be captured into a HIP graph while an eager graph of the same gamma and
     beta is alive; with torch, not while one of the same leaf x is."""
     if _node is None:
         raise ImportError('advmix_amd: _node.so is not there or not for this torch (%s) - build it with `python -m advmix_amd.build`; '

@@ -532,7 +532,7 @@ int advmix_moments_unpack(const uint8_t* codes, const uint8_t* scale, float* x, 
 int advmix_layer_norm_fwd(const void* x, int64_t ldx, const float* gamma, const float* beta, void* y, float* mean, float* rstd,
                           int64_t rows, int C, int dtype, float eps, void* stream);
 /* dx, dgamma, dbeta: any of them NULL = not wanted; dgamma (add & 1) and dbeta (add & 2) are added to what is
- * there, or written (bit 0).  part (when either is wanted): scratch of
+ * there, or written (bit 0); one buffer as both has to be added to (add 3).  part (when either is wanted): scratch of
  * advmix_layer_norm_parts(rows, C, dtype) * 2 * C floats.  The rows are summed in an order that depends on the sizes alone. */
 int advmix_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx, const float* gamma, const float* mean,
                           const float* rstd, void* dx, float* dgamma, float* dbeta, float* part, int add, int64_t rows, int C,

@@ -90,3 +90,12 @@ def test_without_the_torch_side_module(node):
     r = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and 'said:' in r.stdout and 'advmix_amd.build' in r.stdout, (r.stdout, r.stderr)
     assert ('torch 0.1' in r.stdout) == (node != 'None')
+
+
+def test_one_gradient_buffer_as_both_is_only_added_to():
+    """The C entry: a launch that stores two sums to one place is refused before anything is launched."""
+    import ctypes
+    from advmix_amd._lib import lib
+    p = ctypes.c_void_p(4096)                               # never read
+    for add in (0, 1, 2, 4):
+        assert lib.advmix_layer_norm_bwd(p, 8, p, 8, p, p, p, p, p, p, p, add, 4, 8, 0, None) == 1, add
