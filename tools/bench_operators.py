@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""Times of the layer norm and of AdamW: the source of the figures in DESIGN.md's table and beside the kernels.
+"""Times of the layer norm and of AdamW: the source of the figures beside the kernels and in the table of cases.
 
 usage: bench_operators.py                 the rates of this card (a large copy, large matrix products); then each case of
                                           perf/operators.py: an eager pass (host and GPU, one after another) and the same passes

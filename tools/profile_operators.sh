@@ -1,7 +1,7 @@
 #!/bin/bash
-# Times and counters of the layer norm and AdamW (from the repository root, on a machine with the GPU): profile_operators.sh <folder under gpurun_out>
+# Times and counters of the layer norm and AdamW (from the repository root, on a machine with the GPU): profile_operators.sh <output folder>
 # Each counter in a run of its own, kernel trace only.
-R=$PWD; OUT=$R/gpurun_out/$1; mkdir -p $OUT
+mkdir -p "$1"; R=$PWD; OUT=$(cd "$1" && pwd)
 timeout -k 10 120 python3 tools/bench_operators.py > $OUT/cases.log 2>&1 || exit 1
 timeout -k 10 180 python3 tools/bench_operators.py --kernels > $OUT/kernels.log 2>&1 || exit 1
 cd /tmp && export TMPDIR=/tmp
